@@ -11,7 +11,7 @@ Set MURMURA_DISABLE_NATIVE=1 to force the torch path everywhere (debug only).
 from __future__ import annotations
 
 import os
-from typing import Optional, Tuple
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 from torch import Tensor
@@ -219,3 +219,97 @@ def scale_inject(flat: Tensor, lam: float) -> Tensor:
     if _use_native(flat):
         return _EXT.scale_inject(flat, lam)
     return ref.scale_inject(flat, lam)
+
+
+# ------------------------------------------------------------------ K16
+def group_norm_act(x: Tensor, num_groups: int, weight: Optional[Tensor] = None,
+                   bias: Optional[Tensor] = None, eps: float = 1e-5, act: str = "none",
+                   res: Optional[Tensor] = None) -> Tensor:
+    """Group norm, residual and activation in one: y = act(norm(x) * weight +
+    bias + res), differentiable in x, weight, bias and res.
+
+    x is [N, C, H, W] or [N, C], fp32 or bf16; images are worked on channels
+    last (another layout is copied first) and y comes back so. weight and bias
+    ([C]) are of x's type or fp32, res is like x. act: "none", "relu", "silu"
+    or "gelu" (by erf). Statistics are held in fp32 and belong to each sample
+    alone: nothing is kept between calls."""
+    ref.check_group_norm_act(x, num_groups, weight, bias, res)
+    code = ref.check_act(act)
+    if _use_native(x):
+        return _EXT.group_norm_act(x, num_groups, weight, bias, eps, code, res)
+    return ref.group_norm_act(x, num_groups, weight, bias, eps, act, res)
+
+
+# ------------------------------------------------------------------ K17
+def adamw_state(numel: int, device, bits: int = 32):
+    """(exp_avg, exp_avg_sq, step) of an optimizer that has done no step: the
+    moments of ``numel`` parameters in 32 bits, or in 8 with an exponent for
+    each 256 values, and the count of steps on the device."""
+    if bits not in (8, 32):
+        raise ValueError(f"adamw_state: moments are held in 8 or 32 bits, not {bits}")
+
+    def moment():
+        if bits == 32:
+            return torch.zeros(numel, dtype=torch.float32, device=device)
+        return (torch.zeros(numel, dtype=torch.uint8, device=device),
+                torch.zeros(-(-numel // ref.ADAMW_BLOCK), dtype=torch.uint8, device=device))
+
+    return moment(), moment(), torch.zeros(1, dtype=torch.int64, device=device)
+
+
+def adamw_step(params: Union[Tensor, Sequence[Tensor]], grads: Union[Tensor, Sequence[Tensor]],
+               exp_avg: ref.Moment, exp_avg_sq: ref.Moment, step: Tensor,
+               lr: Union[float, Tensor], betas: Tuple[float, float] = (0.9, 0.999),
+               eps: float = 1e-8, weight_decay: float = 0.01, seed: int = 0) -> None:
+    """One AdamW step over all tensors of a model, in place.
+
+    params: a flat vector or the tensors of a model, fp32 or bf16, without gaps
+    or shared memory; grads: as many, of the same shapes, of their type or
+    fp32 (a gradient with other strides than its parameter's is copied first).
+    exp_avg, exp_avg_sq, step: as ``adamw_state`` makes them, the moments in the
+    order of the parameters' memory. lr: a number, or one fp32 value on the device,
+    which a captured step reads anew on each replay; the step's count too lives on
+    the device. bf16 parameters and 8-bit moments are rounded up with the
+    probability of what is cut off, by a hash of (seed, step, place): runs repeat
+    bit for bit, and ranks or nodes that shall differ take different seeds."""
+    params, grads = ref.as_list(params), ref.as_list(grads)
+    if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+        raise ValueError(f"adamw_step: betas lie in [0, 1), got {betas}")
+    if params and _use_native(params[0]):
+        on_device = isinstance(lr, Tensor)
+        _EXT.adamw_step(
+            params, grads, [exp_avg] if isinstance(exp_avg, Tensor) else list(exp_avg),
+            [exp_avg_sq] if isinstance(exp_avg_sq, Tensor) else list(exp_avg_sq), step,
+            0.0 if on_device else lr, lr if on_device else None, betas[0], betas[1], eps,
+            weight_decay, seed & 0xFFFFFFFF)
+        return
+    ref.adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas, eps, weight_decay, seed)
+
+
+def adamw_dequantize(exp_avg: ref.Moment, exp_avg_sq: ref.Moment,
+                     dtype: torch.dtype = torch.float32) -> Tuple[Tensor, Tensor]:
+    """The values of 8-bit moments, in fp32 or bf16 (which holds them as they are)."""
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"adamw_dequantize: fp32 or bf16, not {dtype}")
+    if _use_native(exp_avg[0]):
+        half = dtype == torch.bfloat16
+        return (_EXT.adamw_decode(exp_avg[0], exp_avg[1], True, half),
+                _EXT.adamw_decode(exp_avg_sq[0], exp_avg_sq[1], False, half))
+    return (ref.adamw_decode(*exp_avg, True).to(dtype), ref.adamw_decode(*exp_avg_sq, False).to(dtype))
+
+
+# ------------------------------------------------------------------ K18
+def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: str = "none",
+               res: Optional[Tensor] = None) -> Tensor:
+    """Matrix product with its epilogue: y = act(x @ weight.T + bias + res),
+    differentiable in all four.
+
+    x is [..., K], weight [N, K] (``nn.Linear``'s layout), fp32 or bf16, of one
+    type; bias [N] of that type or fp32; res like y. act: "none", "relu",
+    "silu" or "gelu" (by erf). Sums are fp32, also over bf16 products. For the
+    backward pass silu and gelu keep what they are taken of, in x's type."""
+    ref.check_linear_act(x, weight, bias, res)
+    code = ref.check_act(act)
+    if _use_native(x):
+        return _EXT.linear_act(x, weight, bias, code, res)
+    return ref.linear_act(x, weight, bias, act, res)

@@ -1,0 +1,388 @@
+// AdamW over all tensors of a model in one launch (K17).
+//
+// t is the number of the step. For every parameter p with gradient g:
+//
+//   m = b1*m + (1-b1)*g          v = b2*v + (1-b2)*g*g
+//   p = p*(1 - lr*decay) - lr/(1-b1^t) * m / (sqrt(v)/sqrt(1-b2^t) + eps)
+//
+// The moments lie in the order of the parameters, as one vector of P values
+// each, either in fp32 or in 8 bits. A block of 256 values in 8 bits shares a
+// power of two over its largest value (held as the exponent field e of that
+// value: the scale is 2^(e-126)), and a value below it is kept as
+//
+//   m: sign, 4 bits of exponent, 3 of mantissa   (1+M/8)*2^(E-15), 2^-17 at least
+//   v: 5 bits of exponent, 3 of mantissa         (1+M/8)*2^(E-31), 2^-33 at least
+//
+// with exponent 0 for what has no leading one and all bits set for a NaN (an
+// infinity is kept as one: neither comes back from there in 32 bits either).
+// m and sqrt(v) so have the same range. Codes are rounded up with the
+// probability of what is cut off: 1-b2 of v is a thousandth of it, and steps of
+// an eighth rounded to nearest would never see it. A v above zero never becomes
+// zero, which would make m/sqrt(v) boundless. Parameters in bf16 are rounded
+// the same way, for steps below half of their last bit. The random bits are a
+// hash of (seed, step, place), so a run repeats bit for bit.
+//
+// Every operation is rounded by itself (no contraction): an element's result
+// does not depend on which path, vector width or compiler it went through.
+
+#include "kernel_common.h"
+
+#include <algorithm>
+
+#pragma clang fp contract(off)
+
+namespace mm {
+namespace {
+
+constexpr int NT = 256;
+constexpr int QB = 256;  // values that share a scale
+
+struct Segment {
+  void* p;
+  const void* g;
+  int64_t start;  // place of its first value in the whole vector
+};
+
+// The table travels in the launch's arguments: a captured step needs no copy,
+// and the 4 KB that a launch can carry hold 160 tensors. More take more launches.
+constexpr int MAX_SEGMENTS = 160;
+struct Table {
+  int count;
+  int64_t begin, end;  // the places of this launch
+  Segment s[MAX_SEGMENTS];
+};
+
+struct Moments {  // fp32, or codes and exponents
+  void* m;
+  void* v;
+  unsigned char* me;
+  unsigned char* ve;
+};
+
+struct Hyper {
+  double log_b1, log_b2;
+  float b1, b1c, b2, b2c, eps;
+  double lr, decay;
+  const float* lr_dev;  // in place of lr, where the caller keeps it on the device
+  unsigned int seed;
+  const int64_t* step;  // steps done before this one
+};
+
+// what is the same for all elements of a step
+struct Now {
+  float keep, c1, c2;
+  unsigned int key;
+};
+
+__device__ __forceinline__ Now now_of(const Hyper& h) {
+  const int64_t t = *h.step + 1;
+  const double lr = h.lr_dev ? (double)*h.lr_dev : h.lr;
+  Now n;
+  n.keep = (float)(1.0 - lr * h.decay);
+  n.c1 = (float)(lr / -expm1((double)t * h.log_b1));
+  n.c2 = (float)(1.0 / sqrt(-expm1((double)t * h.log_b2)));
+  n.key = (h.seed * 0x9E3779B1u) ^ ((unsigned int)t * 0x85A308D3u + 0x3C6EF372u);
+  return n;
+}
+
+__device__ __forceinline__ unsigned int hash_of(unsigned int place, unsigned int key) {
+  unsigned int x = place * 0x9E3779B1u + key;
+  x = (x ^ (x >> 16)) * 0x6A09E667u;
+  x = (x ^ (x >> 15)) * 0xBB67AE85u;
+  return x ^ (x >> 16);
+}
+
+__device__ __forceinline__ bf16 dithered_bf16(float f, unsigned int x) {
+  const unsigned int u = __float_as_uint(f);
+  bf16 r;
+  if ((u & 0x7F800000u) == 0x7F800000u)
+    r = round_bf16(f);  // an infinity or a NaN stays what it is
+  else
+    r.v = (unsigned short)((u + ((x * 0xA54FF53Bu) >> 16)) >> 16);
+  return r;
+}
+
+// FIRST: sign + 4 + 3 bits, TOP 15; else 5 + 3 bits, TOP 31
+template <bool FIRST>
+struct Code {
+  static constexpr int TOP = FIRST ? 15 : 31;
+  static constexpr int LOW = -(TOP + 2);
+  static constexpr unsigned int NAN_CODE = 8 * TOP + 7;
+
+  __device__ static __forceinline__ float decode(unsigned int c, int e) {
+    const unsigned int mag = FIRST ? c & 127u : c;
+    const int ex = (int)(mag >> 3);
+    const float f = (float)((mag & 7u) + (ex ? 8u : 0u));
+    float v = ldexpf(f, (ex ? ex - 1 : 0) + LOW + e - 126);
+    if (mag == NAN_CODE) v = __uint_as_float(0x7FC00000u);
+    return FIRST && (c & 128u) ? -v : v;
+  }
+
+  __device__ static __forceinline__ unsigned int encode(float x, int e, unsigned int dither) {
+    const unsigned int bits = __float_as_uint(x), a = bits & 0x7FFFFFFFu;
+    const float s = ldexpf(__uint_as_float(a), 126 - e);
+    unsigned int c;
+    if (s >= (FIRST ? 0x1p-14f : 0x1p-30f))
+      c = ((__float_as_uint(s) + (dither << 4) + 8u) >> 20) - 8 * (127 - TOP);
+    else
+      c = (unsigned int)(s * (FIRST ? 0x1p17f : 0x1p33f) + ((float)dither + 0.5f) * 0x1p-16f);
+    if (!FIRST && a) c = max(c, 1u);
+    if (a >= 0x7F800000u) c = NAN_CODE;
+    return FIRST ? c | (bits >> 31) << 7 : c;
+  }
+};
+
+__device__ __forceinline__ unsigned int finite_bits(float x) {
+  const unsigned int a = __float_as_uint(x) & 0x7FFFFFFFu;
+  return a < 0x7F800000u ? a : 0u;
+}
+
+// the segment that holds a place: the last that starts at or before it
+__device__ __forceinline__ int segment_of(const Table& t, int64_t place) {
+  int lo = 0, hi = t.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (t.s[mid].start <= place)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
+}
+
+// A thread takes 8 values in a row, 32 threads a block of 256 with one scale.
+template <typename T, typename GT, bool EIGHT>
+__global__ __launch_bounds__(NT) void adamw_kernel(Table t, Moments st, Hyper h) {
+  __shared__ Now shared_now;
+  if (threadIdx.x == 0) shared_now = now_of(h);
+  __syncthreads();
+  const Now now = shared_now;
+  const int64_t first = t.begin + ((int64_t)blockIdx.x * NT + threadIdx.x) * 8;
+  const int n = (int)max((int64_t)0, min((int64_t)8, t.end - first));
+  float p[8], g[8], m[8], v[8];
+  T* pp[8];
+  int me = 0, ve = 0;
+  if (EIGHT && n > 0) {
+    me = st.me[first / QB];
+    ve = st.ve[first / QB];
+  }
+  int seg = n > 0 ? segment_of(t, first) : 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    m[i] = v[i] = 0.f;
+    if (i >= n) continue;
+    const int64_t place = first + i;
+    while (seg + 1 < t.count && t.s[seg + 1].start <= place) ++seg;
+    const int64_t at = place - t.s[seg].start;
+    pp[i] = (T*)t.s[seg].p + at;
+    p[i] = to_float(*pp[i]);
+    g[i] = to_float(((const GT*)t.s[seg].g)[at]);
+    if (EIGHT) {
+      m[i] = Code<true>::decode(((const unsigned char*)st.m)[place], me);
+      v[i] = Code<false>::decode(((const unsigned char*)st.v)[place], ve);
+    } else {
+      m[i] = ((const float*)st.m)[place];
+      v[i] = ((const float*)st.v)[place];
+    }
+    m[i] = h.b1 * m[i] + h.b1c * g[i];
+    v[i] = h.b2 * v[i] + h.b2c * (g[i] * g[i]);
+    p[i] = p[i] * now.keep - now.c1 * (m[i] / (sqrtf(v[i]) * now.c2 + h.eps));
+  }
+  if (EIGHT) {
+    unsigned int ma = 0, va = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      ma = max(ma, finite_bits(m[i]));
+      va = max(va, finite_bits(v[i]));
+    }
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      ma = max(ma, (unsigned int)__shfl_xor((int)ma, off, 64));
+      va = max(va, (unsigned int)__shfl_xor((int)va, off, 64));
+    }
+    me = (int)(ma >> 23);
+    ve = (int)(va >> 23);
+    if (n > 0 && (threadIdx.x & 31) == 0) {
+      st.me[first / QB] = (unsigned char)me;
+      st.ve[first / QB] = (unsigned char)ve;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (i >= n) continue;
+    const int64_t place = first + i;
+    const unsigned int x = hash_of((unsigned int)place, now.key);
+    if constexpr (sizeof(T) == 2)
+      *pp[i] = dithered_bf16(p[i], x);
+    else
+      *pp[i] = p[i];
+    if (EIGHT) {
+      ((unsigned char*)st.m)[place] = (unsigned char)Code<true>::encode(m[i], me, x & 0xFFFFu);
+      ((unsigned char*)st.v)[place] = (unsigned char)Code<false>::encode(v[i], ve, x >> 16);
+    } else {
+      ((float*)st.m)[place] = m[i];
+      ((float*)st.v)[place] = v[i];
+    }
+  }
+}
+
+__global__ void adamw_count_kernel(int64_t* step) { *step += 1; }
+
+template <typename O, bool FIRST>
+__global__ __launch_bounds__(NT) void adamw_decode_kernel(const unsigned char* __restrict__ c,
+                                                          const unsigned char* __restrict__ e,
+                                                          int64_t P, O* __restrict__ out) {
+  const int64_t first = ((int64_t)blockIdx.x * NT + threadIdx.x) * 8;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (first + i < P)
+      out[first + i] = from_float<O>(Code<FIRST>::decode(c[first + i], e[first / QB]));
+}
+
+void check_state(const std::vector<Tensor>& s, int64_t P, const at::Device& d) {
+  TORCH_CHECK(s.size() == 1 || s.size() == 2, "adamw_step: a moment is one tensor or two");
+  for (const Tensor& t : s)
+    TORCH_CHECK(t.device() == d && t.is_contiguous(), "adamw_step: moments must be contiguous, "
+                "on the parameters' device");
+  TORCH_CHECK(s[0].numel() == P, "adamw_step: a moment must have a value for each parameter");
+  if (s.size() == 1) {
+    TORCH_CHECK(s[0].scalar_type() == at::kFloat, "adamw_step: a moment of one tensor is fp32");
+  } else {
+    TORCH_CHECK(s[0].scalar_type() == at::kByte && s[1].scalar_type() == at::kByte &&
+                    s[1].numel() == ceil_div(P, QB),
+                "adamw_step: an 8-bit moment is codes [P] and exponents [ceil(P/256)], uint8");
+  }
+}
+
+void adamw_step(const std::vector<Tensor>& params, std::vector<Tensor> grads,
+                const std::vector<Tensor>& exp_avg, const std::vector<Tensor>& exp_avg_sq,
+                const Tensor& step, double lr, const OptTensor& lr_tensor, double b1, double b2,
+                double eps, double decay, int64_t seed) {
+  TORCH_CHECK(!params.empty() && params.size() == grads.size(),
+              "adamw_step: as many gradients as parameters are wanted");
+  const at::Device dev = params[0].device();
+  const auto type = params[0].scalar_type(), gtype = grads[0].scalar_type();
+  TORCH_CHECK(dev.is_cuda() && is_float_type(params[0]), "adamw_step: fp32 or bf16 on a GPU");
+  TORCH_CHECK(gtype == type || gtype == at::kFloat, "adamw_step: gradients are of the parameters' "
+              "type or fp32");
+  const c10::DeviceGuard guard(dev);
+  int64_t P = 0;
+  std::vector<std::pair<const char*, const char*>> spans(params.size());
+  for (size_t i = 0; i < params.size(); ++i) {
+    const Tensor& p = params[i];
+    TORCH_CHECK(p.device() == dev && grads[i].device() == dev && p.scalar_type() == type &&
+                    grads[i].scalar_type() == gtype,
+                "adamw_step: all parameters, and all gradients, must be of one type and device");
+    TORCH_CHECK(p.sizes() == grads[i].sizes(), "adamw_step: a gradient must have its parameter's shape");
+    TORCH_CHECK(p.is_non_overlapping_and_dense(), "adamw_step: a parameter must have no gaps");
+    if (p.strides() != grads[i].strides())  // the same values in the parameter's order
+      grads[i] = at::empty_strided(p.sizes(), p.strides(), grads[i].options()).copy_(grads[i]);
+    spans[i] = {(const char*)p.data_ptr(), (const char*)p.data_ptr() + p.nbytes()};
+    P += p.numel();
+  }
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); ++i)
+    TORCH_CHECK(spans[i - 1].second <= spans[i].first || spans[i].first == spans[i].second,
+                "adamw_step: parameters share memory: pass each once");
+  check_state(exp_avg, P, dev);
+  check_state(exp_avg_sq, P, dev);
+  TORCH_CHECK(exp_avg.size() == exp_avg_sq.size(), "adamw_step: both moments in the same bits");
+  TORCH_CHECK(step.device() == dev && step.scalar_type() == at::kLong && step.numel() == 1,
+              "adamw_step: step is one int64 on the parameters' device");
+  TORCH_CHECK(b1 >= 0 && b1 < 1 && b2 >= 0 && b2 < 1, "adamw_step: betas lie in [0, 1)");
+  if (lr_tensor.has_value())
+    TORCH_CHECK(lr_tensor->device() == dev && lr_tensor->scalar_type() == at::kFloat &&
+                    lr_tensor->numel() == 1,
+                "adamw_step: lr on the device is one fp32 value");
+  const hipStream_t st = stream_of(step);
+  const bool eight = exp_avg.size() == 2;
+  Moments mo{exp_avg[0].data_ptr(), exp_avg_sq[0].data_ptr(), nullptr, nullptr};
+  if (eight) {
+    mo.me = (unsigned char*)exp_avg[1].data_ptr();
+    mo.ve = (unsigned char*)exp_avg_sq[1].data_ptr();
+  }
+  Hyper h;
+  h.log_b1 = log(b1);
+  h.log_b2 = log(b2);
+  h.b1 = (float)b1;
+  h.b1c = (float)(1 - b1);
+  h.b2 = (float)b2;
+  h.b2c = (float)(1 - b2);
+  h.eps = (float)eps;
+  h.lr = lr;
+  h.decay = decay;
+  h.lr_dev = lr_tensor.has_value() ? lr_tensor->data_ptr<float>() : nullptr;
+  h.seed = (unsigned int)seed;
+  h.step = step.data_ptr<int64_t>();
+  // 256 values with one scale must lie within one launch: a tensor that ends inside of them is
+  // listed again at the head of the next table.
+  size_t next = 0;
+  int64_t start = 0;  // place of params[next]
+  Table t;
+  t.begin = 0;
+  while (t.begin < P) {
+    t.count = 0;
+    int64_t at = start;
+    size_t i = next;
+    for (; i < params.size() && t.count < MAX_SEGMENTS; ++i) {
+      if (params[i].numel() == 0) continue;
+      t.s[t.count++] = {params[i].data_ptr(), grads[i].data_ptr(), at};
+      at += params[i].numel();
+    }
+    t.end = i == params.size() ? P : eight ? at / QB * QB : at;
+    TORCH_CHECK(t.end > t.begin, "adamw_step: over ", MAX_SEGMENTS, " tensors within ", QB,
+                " values of 8-bit moments: pass them as one");
+    const int64_t blocks = ceil_div(t.end - t.begin, (int64_t)NT * 8);
+    TORCH_CHECK(blocks < (1LL << 31), "adamw_step: too many values");
+    MM_DISPATCH_TYPE(params[0], {
+      if (gtype == type) {
+        if (eight) adamw_kernel<T, T, true><<<(unsigned)blocks, NT, 0, st>>>(t, mo, h);
+        else adamw_kernel<T, T, false><<<(unsigned)blocks, NT, 0, st>>>(t, mo, h);
+      } else {
+        if (eight) adamw_kernel<T, float, true><<<(unsigned)blocks, NT, 0, st>>>(t, mo, h);
+        else adamw_kernel<T, float, false><<<(unsigned)blocks, NT, 0, st>>>(t, mo, h);
+      }
+    });
+    check_launch("adamw_step");
+    // the next table starts with the tensor that holds place t.end
+    while (next < i && start + params[next].numel() <= t.end) start += params[next++].numel();
+    t.begin = t.end;
+  }
+  adamw_count_kernel<<<1, 1, 0, st>>>(step.data_ptr<int64_t>());
+  check_launch("adamw_step");
+}
+
+Tensor adamw_decode(const Tensor& codes, const Tensor& exps, bool first, bool half) {
+  TORCH_CHECK(codes.is_cuda() && codes.scalar_type() == at::kByte && codes.is_contiguous() &&
+                  exps.scalar_type() == at::kByte && exps.is_contiguous() &&
+                  exps.device() == codes.device() && exps.numel() == ceil_div(codes.numel(), QB),
+              "adamw_dequantize: codes [P] and exponents [ceil(P/256)], uint8");
+  const c10::DeviceGuard guard(codes.device());
+  Tensor out = at::empty(codes.sizes(), codes.options().dtype(half ? at::kBFloat16 : at::kFloat));
+  const int64_t P = codes.numel();
+  if (P == 0) return out;
+  const int64_t blocks = ceil_div(P, (int64_t)NT * 8);
+  TORCH_CHECK(blocks < (1LL << 31), "adamw_dequantize: too many values");
+  const hipStream_t st = stream_of(codes);
+  const auto* c = (const unsigned char*)codes.data_ptr();
+  const auto* e = (const unsigned char*)exps.data_ptr();
+  MM_DISPATCH_TYPE(out, {
+    if (first) adamw_decode_kernel<T, true><<<(unsigned)blocks, NT, 0, st>>>(c, e, P, (T*)out.data_ptr());
+    else adamw_decode_kernel<T, false><<<(unsigned)blocks, NT, 0, st>>>(c, e, P, (T*)out.data_ptr());
+  });
+  check_launch("adamw_dequantize");
+  return out;
+}
+
+}  // namespace
+
+void bind_adamw(pybind11::module_& m) {
+  m.def("adamw_step", &adamw_step, "K17: AdamW over many tensors, moments in fp32 or 8 bits",
+        py::arg("params"), py::arg("grads"), py::arg("exp_avg"), py::arg("exp_avg_sq"),
+        py::arg("step"), py::arg("lr"), py::arg("lr_tensor"), py::arg("b1"), py::arg("b2"),
+        py::arg("eps"), py::arg("decay"), py::arg("seed"));
+  m.def("adamw_decode", &adamw_decode, "K17: the values of an 8-bit moment", py::arg("codes"),
+        py::arg("exps"), py::arg("first"), py::arg("half"));
+}
+
+}  // namespace mm

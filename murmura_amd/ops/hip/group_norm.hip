@@ -1,0 +1,570 @@
+// Group norm with residual and activation over channels-last images (K16).
+//
+// x is [N, R, C] in memory, R pixels of C channels; group g of sample n holds
+// R * C/G values. With mean, rstd over a group and xhat = (x - mean) * rstd:
+//
+//   z = xhat * gamma + beta (+ res),  y = act(z)
+//   dz = dy * act'(z),  dres = dz,  dbeta = sum dz,  dgamma = sum dz * xhat
+//   dx = rstd * (dz*gamma - avg(dz*gamma) - xhat * avg(dz*gamma*xhat))
+//
+// A thread owns V channels (one memory transaction) and walks over rows, so
+// that every load is whole and the channels' sums stay in registers. Sums run
+// rows of a thread -> lanes of a wave -> waves of a block -> chunks, always in
+// the same order: no atomics, the same bits on every run. All statistics are
+// fp32; a variance is taken around its own mean, chunks are joined by their
+// counts, so that a level far above the spread costs no digits.
+
+#include "kernel_common.h"
+
+namespace mm {
+namespace {
+
+constexpr int NT = 256;          // threads of a block
+constexpr int NW = NT / 64;      // its waves
+constexpr int K = 8;             // rows that a thread holds
+constexpr int MAX_TILE = 64 * 8; // channels of a tile: 64 lanes of 8
+
+struct Shape {
+  int64_t R;    // pixels of a sample
+  int C, G, Cg; // channels, groups, channels of a group
+  int lanes;    // log2 of the lanes that lie side by side along the channels
+  int tiles;    // channel tiles of (1 << lanes) * V
+  int S;        // row chunks of (NT >> lanes) * K
+};
+
+struct Place {
+  int64_t n, row0, rows;  // sample; first row of the chunk; rows in it
+  int tile, chunk, col, c, lane_row, step;
+  bool active;
+};
+
+template <int V>
+__device__ __forceinline__ Place place_of(const Shape& s) {
+  Place p;
+  const int64_t b = blockIdx.x;
+  p.chunk = (int)(b % s.S);
+  p.tile = (int)((b / s.S) % s.tiles);
+  p.n = b / ((int64_t)s.S * s.tiles);
+  p.step = NT >> s.lanes;
+  p.row0 = (int64_t)p.chunk * p.step * K;
+  p.rows = min((int64_t)p.step * K, s.R - p.row0);
+  p.col = threadIdx.x & ((1 << s.lanes) - 1);
+  p.lane_row = threadIdx.x >> s.lanes;
+  p.c = (p.tile * (1 << s.lanes) + p.col) * V;
+  p.active = p.c < s.C;
+  return p;
+}
+
+// Sums `acc` over the rows of the block; part[wave][channel of the tile] holds
+// what the waves have, the caller adds them after the barrier.
+template <int V>
+__device__ __forceinline__ void rows_to_waves(float (&acc)[V], int lanes, int col, float* part) {
+  for (int off = 1 << lanes; off < 64; off <<= 1) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[v] += __shfl_xor(acc[v], off, 64);
+  }
+  const int tile = (1 << lanes) * V;
+  if ((threadIdx.x & 63) < (1 << lanes)) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) part[(threadIdx.x >> 6) * tile + col * V + v] = acc[v];
+  }
+}
+
+__device__ __forceinline__ float over_waves(const float* part, int tile, int c) {
+  float s = 0.f;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) s += part[w * tile + c];
+  return s;
+}
+
+// (mean, sum of squares around it) of each channel over a chunk of rows
+template <typename T, int V>
+__global__ __launch_bounds__(NT) void gn_stats_kernel(const T* __restrict__ x, Shape s,
+                                                      float2* __restrict__ ws) {
+  __shared__ float part[NW * MAX_TILE];
+  __shared__ float mean[MAX_TILE];
+  const Place p = place_of<V>(s);
+  const int tile = (1 << s.lanes) * V;
+  const float inv = 1.f / (float)p.rows;
+  Vec<T, V> val[K];
+  float acc[V] = {};
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const int64_t r = p.lane_row + i * p.step;
+    if (p.active && r < p.rows) {
+      val[i] = *(const Vec<T, V>*)(x + (p.n * s.R + p.row0 + r) * s.C + p.c);
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[v] += to_float(val[i].e[v]);
+    }
+  }
+  rows_to_waves<V>(acc, s.lanes, p.col, part);
+  __syncthreads();
+  for (int c = threadIdx.x; c < tile; c += NT) mean[c] = over_waves(part, tile, c) * inv;
+  __syncthreads();
+#pragma unroll
+  for (int v = 0; v < V; ++v) acc[v] = 0.f;
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const int64_t r = p.lane_row + i * p.step;
+    if (p.active && r < p.rows) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const float d = to_float(val[i].e[v]) - mean[p.col * V + v];
+        acc[v] += d * d;
+      }
+    }
+  }
+  rows_to_waves<V>(acc, s.lanes, p.col, part);
+  __syncthreads();
+  for (int c = threadIdx.x; c < tile; c += NT) {
+    const int cc = p.tile * tile + c;
+    if (cc < s.C)
+      ws[(p.n * s.S + p.chunk) * s.C + cc] = make_float2(mean[c], over_waves(part, tile, c));
+  }
+}
+
+__device__ __forceinline__ float block_sum(float v, float* lds) {
+  v = wave_sum(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  float s = 0.f;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) s += lds[w];
+  return s;
+}
+
+// one block a group: joins the chunks' statistics
+__global__ __launch_bounds__(NT) void gn_join_stats_kernel(const float2* __restrict__ ws, Shape s,
+                                                           float eps, float* __restrict__ mean,
+                                                           float* __restrict__ rstd) {
+  __shared__ float lds[NW];
+  const int64_t n = blockIdx.x / s.G;
+  const int g = blockIdx.x % s.G;
+  const int64_t chunk_rows = (int64_t)(NT >> s.lanes) * K;
+  const float2* w = ws + n * s.S * s.C + g * s.Cg;
+  const int64_t entries = (int64_t)s.S * s.Cg;
+  float sum = 0.f;
+  for (int64_t e = threadIdx.x; e < entries; e += NT) {
+    const int64_t k = e / s.Cg;
+    sum += w[k * s.C + e % s.Cg].x * (float)min(chunk_rows, s.R - k * chunk_rows);
+  }
+  const float inv = 1.f / ((float)s.R * (float)s.Cg);
+  const float mu = block_sum(sum, lds) * inv;
+  float m2 = 0.f;
+  for (int64_t e = threadIdx.x; e < entries; e += NT) {
+    const int64_t k = e / s.Cg;
+    const float2 q = w[k * s.C + e % s.Cg];
+    const float d = q.x - mu;
+    m2 += q.y + d * d * (float)min(chunk_rows, s.R - k * chunk_rows);
+  }
+  m2 = block_sum(m2, lds);
+  if (threadIdx.x == 0) {
+    mean[blockIdx.x] = mu;
+    rstd[blockIdx.x] = 1.f / sqrtf(m2 * inv + eps);
+  }
+}
+
+// the affine map of a thread's channels
+template <int V>
+struct Affine {
+  float mu[V], rs[V], ga[V], be[V];
+  __device__ __forceinline__ void load(const Shape& s, const Place& p, const float* mean,
+                                       const float* rstd, const void* gamma, const void* beta,
+                                       bool wf) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int g = (p.c + v) / s.Cg;
+      mu[v] = mean[p.n * s.G + g];
+      rs[v] = rstd[p.n * s.G + g];
+      ga[v] = load_param(gamma, p.c + v, wf, 1.f);
+      be[v] = load_param(beta, p.c + v, wf, 0.f);
+    }
+  }
+  __device__ __forceinline__ float xhat(float x, int v) const { return (x - mu[v]) * rs[v]; }
+};
+
+template <typename T, int V, int ACT>
+__global__ __launch_bounds__(NT) void gn_apply_kernel(
+    const T* __restrict__ x, const T* __restrict__ res, Shape s, const float* __restrict__ mean,
+    const float* __restrict__ rstd, const void* __restrict__ gamma, const void* __restrict__ beta,
+    bool wf, T* __restrict__ y) {
+  const Place p = place_of<V>(s);
+  if (!p.active) return;
+  Affine<V> a;
+  a.load(s, p, mean, rstd, gamma, beta, wf);
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const int64_t r = p.lane_row + i * p.step;
+    if (r >= p.rows) break;
+    const int64_t at = (p.n * s.R + p.row0 + r) * s.C + p.c;
+    const Vec<T, V> xv = *(const Vec<T, V>*)(x + at);
+    Vec<T, V> rv, yv;
+    if (res) rv = *(const Vec<T, V>*)(res + at);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float z = a.xhat(to_float(xv.e[v]), v) * a.ga[v] + a.be[v];
+      if (res) z += to_float(rv.e[v]);
+      yv.e[v] = from_float<T>(act_fwd<ACT>(z));
+    }
+    *(Vec<T, V>*)(y + at) = yv;
+  }
+}
+
+// (sum dz, sum dz * xhat) of each channel over a chunk of rows; dres = dz
+template <typename T, int V, int ACT>
+__global__ __launch_bounds__(NT) void gn_bwd_sums_kernel(
+    const T* __restrict__ x, const T* __restrict__ dy, const T* __restrict__ res, Shape s,
+    const float* __restrict__ mean, const float* __restrict__ rstd, const void* __restrict__ gamma,
+    const void* __restrict__ beta, bool wf, T* __restrict__ dres, float2* __restrict__ ws) {
+  __shared__ float part[2][NW * MAX_TILE];
+  const Place p = place_of<V>(s);
+  const int tile = (1 << s.lanes) * V;
+  float sz[V] = {}, sx[V] = {};
+  if (p.active) {
+    Affine<V> a;
+    a.load(s, p, mean, rstd, gamma, beta, wf);
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+      const int64_t r = p.lane_row + i * p.step;
+      if (r >= p.rows) break;
+      const int64_t at = (p.n * s.R + p.row0 + r) * s.C + p.c;
+      const Vec<T, V> xv = *(const Vec<T, V>*)(x + at);
+      const Vec<T, V> dv = *(const Vec<T, V>*)(dy + at);
+      Vec<T, V> rv, dr;
+      if (res) rv = *(const Vec<T, V>*)(res + at);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const float xh = a.xhat(to_float(xv.e[v]), v);
+        float z = xh * a.ga[v] + a.be[v];
+        if (res) z += to_float(rv.e[v]);
+        const float dz = act_bwd<ACT>(to_float(dv.e[v]), z);
+        sz[v] += dz;
+        sx[v] += dz * xh;
+        dr.e[v] = from_float<T>(dz);
+      }
+      if (dres) *(Vec<T, V>*)(dres + at) = dr;
+    }
+  }
+  rows_to_waves<V>(sz, s.lanes, p.col, part[0]);
+  rows_to_waves<V>(sx, s.lanes, p.col, part[1]);
+  __syncthreads();
+  for (int c = threadIdx.x; c < tile; c += NT) {
+    const int cc = p.tile * tile + c;
+    if (cc < s.C)
+      ws[(p.n * s.S + p.chunk) * s.C + cc] =
+          make_float2(over_waves(part[0], tile, c), over_waves(part[1], tile, c));
+  }
+}
+
+// one block a group: avg(dz*gamma), avg(dz*gamma*xhat)
+__global__ __launch_bounds__(NT) void gn_join_sums_kernel(const float2* __restrict__ ws, Shape s,
+                                                          const void* __restrict__ gamma, bool wf,
+                                                          float2* __restrict__ avg) {
+  __shared__ float lds[NW];
+  const int64_t n = blockIdx.x / s.G;
+  const int g = blockIdx.x % s.G;
+  const float2* w = ws + n * s.S * s.C + g * s.Cg;
+  const int64_t entries = (int64_t)s.S * s.Cg;
+  float sz = 0.f, sx = 0.f;
+  for (int64_t e = threadIdx.x; e < entries; e += NT) {
+    const int64_t k = e / s.Cg;
+    const int c = (int)(e % s.Cg);
+    const float2 q = w[k * s.C + c];
+    const float ga = load_param(gamma, g * s.Cg + c, wf, 1.f);
+    sz += q.x * ga;
+    sx += q.y * ga;
+  }
+  const float inv = 1.f / ((float)s.R * (float)s.Cg);
+  sz = block_sum(sz, lds) * inv;
+  sx = block_sum(sx, lds) * inv;
+  if (threadIdx.x == 0) avg[blockIdx.x] = make_float2(sz, sx);
+}
+
+template <typename T, int V, int ACT>
+__global__ __launch_bounds__(NT) void gn_bwd_dx_kernel(
+    const T* __restrict__ x, const T* __restrict__ dy, const T* __restrict__ res, Shape s,
+    const float* __restrict__ mean, const float* __restrict__ rstd, const float2* __restrict__ avg,
+    const void* __restrict__ gamma, const void* __restrict__ beta, bool wf, T* __restrict__ dx) {
+  const Place p = place_of<V>(s);
+  if (!p.active) return;
+  Affine<V> a;
+  a.load(s, p, mean, rstd, gamma, beta, wf);
+  float2 m[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) m[v] = avg[p.n * s.G + (p.c + v) / s.Cg];
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const int64_t r = p.lane_row + i * p.step;
+    if (r >= p.rows) break;
+    const int64_t at = (p.n * s.R + p.row0 + r) * s.C + p.c;
+    const Vec<T, V> xv = *(const Vec<T, V>*)(x + at);
+    const Vec<T, V> dv = *(const Vec<T, V>*)(dy + at);
+    Vec<T, V> rv, out;
+    if (res) rv = *(const Vec<T, V>*)(res + at);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const float xh = a.xhat(to_float(xv.e[v]), v);
+      float z = xh * a.ga[v] + a.be[v];
+      if (res) z += to_float(rv.e[v]);
+      const float dz = act_bwd<ACT>(to_float(dv.e[v]), z);
+      out.e[v] = from_float<T>(a.rs[v] * (dz * a.ga[v] - m[v].x - xh * m[v].y));
+    }
+    *(Vec<T, V>*)(dx + at) = out;
+  }
+}
+
+// dgamma, dbeta: 64 channels a block, its waves over the rows of ws [rows, C]
+__global__ __launch_bounds__(1024) void gn_bwd_params_kernel(const float2* __restrict__ ws,
+                                                             int64_t rows, int C, bool wf,
+                                                             void* __restrict__ dgamma,
+                                                             void* __restrict__ dbeta) {
+  __shared__ float2 lds[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = blockIdx.x * 64 + lane;
+  float sz = 0.f, sx = 0.f;
+  if (c < C) {
+    for (int64_t r = wave; r < rows; r += 16) {
+      const float2 q = ws[r * C + c];
+      sz += q.x;
+      sx += q.y;
+    }
+  }
+  lds[wave][lane] = make_float2(sz, sx);
+  __syncthreads();
+  if (wave == 0 && c < C) {
+    for (int w = 1; w < 16; ++w) {
+      sz += lds[w][lane].x;
+      sx += lds[w][lane].y;
+    }
+    if (dgamma) store_param(dgamma, c, wf, sx);
+    if (dbeta) store_param(dbeta, c, wf, sz);
+  }
+}
+
+// ------------------------------------------------------------------ host
+struct Image {
+  int64_t N, R;
+  int C;
+};
+
+Image image_of(const Tensor& x) {
+  return {x.size(0), x.dim() == 4 ? x.size(2) * x.size(3) : 1, (int)x.size(1)};
+}
+
+Tensor channels_last(const Tensor& t) {
+  return t.dim() == 4 ? t.contiguous(at::MemoryFormat::ChannelsLast) : t.contiguous();
+}
+
+Tensor like(const Tensor& t) {
+  return at::empty_like(
+      t, t.options(), t.dim() == 4 ? at::MemoryFormat::ChannelsLast : at::MemoryFormat::Contiguous);
+}
+
+void check_args(const Tensor& x, int64_t groups, const Tensor& w, const Tensor& b, const Tensor& res,
+                int64_t act) {
+  TORCH_CHECK(x.is_cuda() && is_float_type(x), "group_norm_act: x must be fp32 or bf16 on a GPU");
+  TORCH_CHECK(x.dim() == 2 || x.dim() == 4, "group_norm_act: x must be [N, C] or [N, C, H, W]");
+  const int64_t C = x.size(1);
+  TORCH_CHECK(groups > 0 && C > 0 && C % groups == 0 && C < (1 << 24),
+              "group_norm_act: num_groups must divide the channels");
+  TORCH_CHECK(act >= 0 && act <= 3, "group_norm_act: unknown activation");
+  for (const Tensor* p : {&w, &b}) {
+    if (!p->defined()) continue;
+    TORCH_CHECK(p->device() == x.device() && p->dim() == 1 && p->size(0) == C,
+                "group_norm_act: weight and bias must be [C] on x's device");
+    TORCH_CHECK(p->scalar_type() == at::kFloat || p->scalar_type() == x.scalar_type(),
+                "group_norm_act: weight and bias must be fp32 or of x's type");
+  }
+  TORCH_CHECK(!w.defined() || !b.defined() || w.scalar_type() == b.scalar_type(),
+              "group_norm_act: weight and bias must be of one type");
+  if (res.defined())
+    TORCH_CHECK(res.device() == x.device() && res.scalar_type() == x.scalar_type() &&
+                    res.sizes() == x.sizes(),
+                "group_norm_act: res must be like x");
+}
+
+bool aligned(std::initializer_list<const void*> ptrs, size_t to) {
+  for (const void* p : ptrs)
+    if ((uintptr_t)p % to) return false;
+  return true;
+}
+
+// channels of one transaction: 16 bytes where the rows and all pointers allow it, else 8 or 4
+// bytes (two values), else one value
+int vector_of(int C, int64_t elem, std::initializer_list<const void*> ptrs) {
+  for (int64_t v = 16 / elem; v > 1; v >>= 1)
+    if (C % v == 0 && aligned(ptrs, v * elem)) return (int)v;
+  return 1;
+}
+
+Shape shape_of(const Image& im, int64_t groups, int V) {
+  Shape s;
+  s.R = im.R;
+  s.C = im.C;
+  s.G = (int)groups;
+  s.Cg = im.C / s.G;
+  s.lanes = 0;
+  while (s.lanes < 6 && (1 << s.lanes) * V < s.C) ++s.lanes;
+  s.tiles = (int)ceil_div(s.C, (int64_t)(1 << s.lanes) * V);
+  const int64_t S = ceil_div(s.R, (int64_t)(NT >> s.lanes) * K);
+  TORCH_CHECK(im.N * s.tiles * S < (1LL << 31) && im.N * groups < (1LL << 31),
+              "group_norm_act: too many blocks");
+  s.S = (int)S;
+  return s;
+}
+
+#define GN_DISPATCH_VEC(V_VALUE, ...)                                      \
+  switch (V_VALUE) {                                                       \
+    case 8: { constexpr int V = sizeof(T) == 2 ? 8 : 4; __VA_ARGS__; } break; \
+    case 4: { constexpr int V = 4; __VA_ARGS__; } break;                   \
+    case 2: { constexpr int V = 2; __VA_ARGS__; } break;                   \
+    default: { constexpr int V = 1; __VA_ARGS__; } break;                  \
+  }
+
+const void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+struct Forward {
+  Tensor y, x, w, b, res, mean, rstd;  // the result, and what the backward pass reads
+};
+
+void normalise(Forward& f, int64_t groups, double eps, int64_t act) {
+  const Tensor &x = f.x, &w = f.w, &b = f.b, &res = f.res;
+  const Image im = image_of(x);
+  Tensor& y = f.y = like(x);
+  Tensor& mean = f.mean = at::empty({im.N, groups}, x.options().dtype(at::kFloat));
+  Tensor& rstd = f.rstd = at::empty_like(mean);
+  if (x.numel() == 0) return;
+  const bool wf = (w.defined() ? w : b.defined() ? b : x).scalar_type() == at::kFloat;
+  const int vec = vector_of(im.C, x.element_size(), {ptr(x), ptr(res), ptr(y)});
+  const Shape s = shape_of(im, groups, vec);
+  const hipStream_t st = stream_of(x);
+  Tensor ws = at::empty({im.N * s.S * s.C * 2}, mean.options());
+  const unsigned blocks = (unsigned)(im.N * s.tiles * s.S);
+  MM_DISPATCH_TYPE(x, GN_DISPATCH_VEC(vec, {
+    gn_stats_kernel<T, V><<<blocks, NT, 0, st>>>((const T*)ptr(x), s, (float2*)ws.data_ptr());
+    gn_join_stats_kernel<<<(unsigned)(im.N * groups), NT, 0, st>>>(
+        (const float2*)ws.data_ptr(), s, (float)eps, mean.data_ptr<float>(), rstd.data_ptr<float>());
+    MM_DISPATCH_ACT(act, (gn_apply_kernel<T, V, ACT><<<blocks, NT, 0, st>>>(
+        (const T*)ptr(x), (const T*)ptr(res), s, mean.data_ptr<float>(), rstd.data_ptr<float>(),
+        ptr(w), ptr(b), wf, (T*)y.data_ptr())));
+  }));
+  check_launch("group_norm_act");
+}
+
+struct Grads {
+  Tensor dx, dw, db, dres;
+};
+
+Grads backward_of(const Tensor& dy, const Tensor& x, int64_t groups, const Tensor& w,
+                  const Tensor& b, int64_t act, const Tensor& res, const Tensor& mean,
+                  const Tensor& rstd, bool need_dx, bool need_dw, bool need_db, bool need_dres) {
+  const Image im = image_of(x);
+  Grads g;
+  if (need_dx) g.dx = like(x);
+  if (need_dw) g.dw = at::empty_like(w);
+  if (need_db) g.db = at::empty_like(b);
+  if (need_dres) g.dres = like(x);
+  if (x.numel() == 0) {
+    if (need_dw) g.dw.zero_();
+    if (need_db) g.db.zero_();
+    return g;
+  }
+  const bool wf = (w.defined() ? w : b.defined() ? b : x).scalar_type() == at::kFloat;
+  const int vec = vector_of(im.C, x.element_size(),
+                            {ptr(x), ptr(dy), ptr(res), ptr(g.dx), ptr(g.dres)});
+  const Shape s = shape_of(im, groups, vec);
+  const hipStream_t st = stream_of(x);
+  Tensor ws = at::empty({im.N * s.S * s.C * 2}, mean.options());
+  Tensor avg = at::empty({im.N * groups * 2}, mean.options());
+  const unsigned blocks = (unsigned)(im.N * s.tiles * s.S);
+  MM_DISPATCH_TYPE(x, GN_DISPATCH_VEC(vec, {
+    MM_DISPATCH_ACT(act, (gn_bwd_sums_kernel<T, V, ACT><<<blocks, NT, 0, st>>>(
+        (const T*)ptr(x), (const T*)ptr(dy), (const T*)ptr(res), s, mean.data_ptr<float>(),
+        rstd.data_ptr<float>(), ptr(w), ptr(b), wf, (T*)ptr(g.dres), (float2*)ws.data_ptr())));
+    if (need_dx) {
+      gn_join_sums_kernel<<<(unsigned)(im.N * groups), NT, 0, st>>>(
+          (const float2*)ws.data_ptr(), s, ptr(w), wf, (float2*)avg.data_ptr());
+      MM_DISPATCH_ACT(act, (gn_bwd_dx_kernel<T, V, ACT><<<blocks, NT, 0, st>>>(
+          (const T*)ptr(x), (const T*)ptr(dy), (const T*)ptr(res), s, mean.data_ptr<float>(),
+          rstd.data_ptr<float>(), (const float2*)avg.data_ptr(), ptr(w), ptr(b), wf,
+          (T*)g.dx.data_ptr())));
+    }
+  }));
+  if (need_dw || need_db)
+    gn_bwd_params_kernel<<<(unsigned)ceil_div(s.C, 64), 1024, 0, st>>>(
+        (const float2*)ws.data_ptr(), im.N * s.S, s.C, wf, (void*)ptr(g.dw), (void*)ptr(g.db));
+  check_launch("group_norm_act backward");
+  return g;
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
+
+Forward forward_of(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& res,
+                   int64_t groups, double eps, int64_t act) {
+  Forward f;
+  f.x = channels_last(x);
+  f.w = w.defined() ? w.contiguous() : w;
+  f.b = b.defined() ? b.contiguous() : b;
+  f.res = res.defined() ? channels_last(res) : res;
+  normalise(f, groups, eps, act);
+  return f;
+}
+
+class GroupNormAct : public torch::autograd::Function<GroupNormAct> {
+ public:
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& weight,
+                        const OptTensor& bias, const OptTensor& residual, int64_t groups,
+                        double eps, int64_t act) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor()),
+                 res = residual.value_or(Tensor());
+    const Forward f = forward_of(x, w, b, res, groups, eps, act);
+    // without an activation the backward pass never looks at the residual
+    ctx->save_for_backward(
+        {f.x, f.w, f.b, act == ACT_NONE ? Tensor() : f.res, f.mean, f.rstd});
+    ctx->saved_data["groups"] = groups;
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["needs"] = (int64_t)(x.requires_grad() | wants_grad(w) << 1 |
+                                         wants_grad(b) << 2 | wants_grad(res) << 3);
+    return f.y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(),
+                "group_norm_act has no second derivative (create_graph=True)");
+    const auto saved = ctx->get_saved_variables();
+    const int64_t needs = ctx->saved_data["needs"].toInt();
+    const c10::DeviceGuard guard(saved[0].device());
+    Grads g = backward_of(channels_last(grads[0]), saved[0], ctx->saved_data["groups"].toInt(),
+                          saved[1], saved[2], ctx->saved_data["act"].toInt(), saved[3], saved[4],
+                          saved[5], needs & 1, needs & 2, needs & 4, needs & 8);
+    return {g.dx, g.dw, g.db, g.dres, Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor group_norm_act(const Tensor& x, int64_t groups, const OptTensor& weight,
+                      const OptTensor& bias, double eps, int64_t act, const OptTensor& residual) {
+  const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor()),
+               res = residual.value_or(Tensor());
+  check_args(x, groups, w, b, res, act);
+  const c10::DeviceGuard guard(x.device());
+  if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b) || wants_grad(res)))
+    return GroupNormAct::apply(x, weight, bias, residual, groups, eps, act);
+  return forward_of(x, w, b, res, groups, eps, act).y;
+}
+
+}  // namespace
+
+void bind_group_norm(pybind11::module_& m) {
+  m.def("group_norm_act", &group_norm_act,
+        "K16: channels-last group norm (+residual) (+activation), differentiable",
+        py::arg("x"), py::arg("num_groups"), py::arg("weight") = py::none(),
+        py::arg("bias") = py::none(), py::arg("eps") = 1e-5, py::arg("act") = 0,
+        py::arg("res") = py::none());
+}
+
+}  // namespace mm

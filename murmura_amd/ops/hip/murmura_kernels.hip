@@ -2105,7 +2105,17 @@ Tensor conv3x3s1_wrw(Tensor x, Tensor dy) {
 
 }  // namespace
 
+// the kernels of the local training step, in files of their own
+namespace mm {
+void bind_group_norm(pybind11::module_& m);
+void bind_adamw(pybind11::module_& m);
+void bind_linear_act(pybind11::module_& m);
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  mm::bind_group_norm(m);
+  mm::bind_adamw(m);
+  mm::bind_linear_act(m);
   m.def("bn_fwd_train", &bn_fwd_train,
         "K14: fused NHWC BatchNorm(+ReLU)(+residual) training forward -> "
         "(y, mean, invstd)",

@@ -11,7 +11,8 @@ All ops operate on flat state vectors [P] or stacked states [m, P]
 
 from __future__ import annotations
 
-from typing import Optional, Tuple
+import math
+from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
 from torch import Tensor
@@ -182,3 +183,229 @@ def gaussian_inject(flat: Tensor, noise_std: float, seed: int, offset: int = 0) 
 def scale_inject(flat: Tensor, lam: float) -> Tensor:
     """attacked = lam * flat (reference: attacks/directed.py:79-89)."""
     return flat * lam
+
+
+# ------------------------------------------------- the local training step
+ACTIVATIONS = ("none", "relu", "silu", "gelu")
+
+
+def check_act(act: str) -> int:
+    """The number of an activation's name, as the kernels know it."""
+    if act not in ACTIVATIONS:
+        raise ValueError(f"unknown activation {act!r}; options: {list(ACTIVATIONS)}")
+    return ACTIVATIONS.index(act)
+
+
+def _activate(z: Tensor, act: str) -> Tensor:
+    if act == "relu":
+        return torch.relu(z)
+    if act == "silu":
+        return z * torch.sigmoid(z)
+    if act == "gelu":
+        return 0.5 * z * (1.0 + torch.erf(z * 0.7071067811865476))
+    return z
+
+
+def _wide(t: Tensor) -> Tensor:
+    return t if t.dtype == torch.float64 else t.float()
+
+
+# ---------------------------------------------------------------- K16
+def check_group_norm_act(x: Tensor, num_groups: int, weight: Optional[Tensor],
+                         bias: Optional[Tensor], res: Optional[Tensor]) -> None:
+    if x.dim() not in (2, 4):
+        raise ValueError(f"group_norm_act: x must be [N, C] or [N, C, H, W], got {tuple(x.shape)}")
+    c = x.shape[1]
+    if num_groups < 1 or c < 1 or c % num_groups:
+        raise ValueError(f"group_norm_act: {num_groups} groups do not divide {c} channels")
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is not None and (p.shape != (c,) or p.device != x.device
+                              or p.dtype not in (x.dtype, torch.float32)):
+            raise ValueError(f"group_norm_act: {name} must be [{c}] on {x.device}, "
+                             f"{x.dtype} or fp32")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError("group_norm_act: weight and bias must be of one type")
+    if res is not None and (res.shape != x.shape or res.device != x.device
+                            or res.dtype != x.dtype):
+        raise ValueError("group_norm_act: res must have x's shape, type and device")
+
+
+def group_norm_act(x: Tensor, num_groups: int, weight: Optional[Tensor] = None,
+                   bias: Optional[Tensor] = None, eps: float = 1e-5, act: str = "none",
+                   res: Optional[Tensor] = None) -> Tensor:
+    """y = act((x - mean) / sqrt(var + eps) * weight + bias (+ res)), mean and
+    (biased) variance over the pixels and channels of each group, in 32 bits
+    and rounded once."""
+    check_group_norm_act(x, num_groups, weight, bias, res)
+    check_act(act)
+    n, c = x.shape[:2]
+    g = _wide(x).reshape(n, num_groups, -1)
+    if g.shape[2] and n:
+        d = g - g.mean(2, keepdim=True)
+        g = d / torch.sqrt(d.square().mean(2, keepdim=True) + eps)
+    z = g.reshape(x.shape)
+    per_channel = (1, c) + (1,) * (x.dim() - 2)
+    if weight is not None:
+        z = z * _wide(weight).view(per_channel)
+    if bias is not None:
+        z = z + _wide(bias).view(per_channel)
+    if res is not None:
+        z = z + _wide(res)
+    y = _activate(z, act).to(x.dtype)
+    return y.contiguous(memory_format=torch.channels_last) if x.dim() == 4 else y
+
+
+# ---------------------------------------------------------------- K17
+#: a moment: fp32 [P], or (codes [P], exponents [ceil(P/256)]) in uint8
+Moment = Union[Tensor, Tuple[Tensor, Tensor]]
+ADAMW_BLOCK = 256
+
+
+def _pow2(e: Tensor) -> Tensor:
+    """2**e in 64 bits for whole e, from its bits."""
+    return ((e.to(torch.int64) + 1023) << 52).view(torch.float64)
+
+
+def _moment_form(first: bool) -> Tuple[int, float]:
+    """(exponent of the code whose mantissa is bare, smallest code's value)."""
+    return (15, 2.0 ** -17) if first else (31, 2.0 ** -33)
+
+
+def adamw_decode(codes: Tensor, exps: Tensor, first: bool) -> Tensor:
+    """fp32 values of an 8-bit moment (the format stands at K17's kernel)."""
+    top, least = _moment_form(first)
+    c = codes.to(torch.int64)
+    mag = c & 127 if first else c
+    e = mag >> 3
+    value = ((mag & 7) + 8 * (e > 0)).double() * least * _pow2((e - 1).clamp_min(0))
+    value = value.masked_fill(mag == 8 * top + 7, math.nan)
+    if first:
+        value = torch.where(c > 127, -value, value)
+    scale = _pow2(exps.to(torch.int64) - 126).repeat_interleave(ADAMW_BLOCK)[: codes.numel()]
+    return (value * scale).float()
+
+
+def adamw_encode(x: Tensor, first: bool, dither: Tensor) -> Tuple[Tensor, Tensor]:
+    """(codes, exponents) of fp32 values [P]; dither: 16 random bits a value."""
+    top, least = _moment_form(first)
+    a = x.abs()
+    finite = torch.isfinite(x)
+    blocks = torch.nn.functional.pad(a.masked_fill(~finite, 0.0), (0, -x.numel() % ADAMW_BLOCK))
+    exps = blocks.view(-1, ADAMW_BLOCK).amax(1).view(torch.int32) >> 23
+    scale = _pow2(exps - 126).repeat_interleave(ADAMW_BLOCK)[: x.numel()]
+    s = (a.double() / scale).float()
+    whole = ((s.view(torch.int32).to(torch.int64) + (dither << 4) + 8) >> 20) - 8 * (127 - top)
+    small = (s / least + (dither.float() + 0.5) / 65536).floor().nan_to_num(0.0).clamp(0, 255)
+    code = torch.where(s >= 8 * least, whole, small.to(torch.int64))
+    if not first:
+        code = torch.where(a > 0, code.clamp_min(1), code)
+    code = torch.where(finite, code, 8 * top + 7)
+    if first:
+        code = code + 128 * torch.signbit(x)
+    return code.to(torch.uint8), exps.to(torch.uint8)
+
+
+def adamw_dither(numel: int, seed: int, t: int, device) -> Tuple[Tensor, Tensor, Tensor]:
+    """16 random bits for the first moment, the second and the parameter at
+    each place, from a hash of (seed, step, place)."""
+    low = 0xFFFFFFFF
+    key = ((seed & low) * 0x9E3779B1 & low) ^ (((t & low) * 0x85A308D3 + 0x3C6EF372) & low)
+    x = (torch.arange(numel, dtype=torch.int64, device=device) & low) * 0x9E3779B1 + key & low
+    x = (x ^ x >> 16) * 0x6A09E667 & low
+    x = (x ^ x >> 15) * 0xBB67AE85 & low
+    x = x ^ x >> 16
+    return x & 0xFFFF, x >> 16, (x * 0xA54FF53B & low) >> 16
+
+
+def as_list(t: Union[Tensor, Sequence[Tensor]]) -> List[Tensor]:
+    return [t] if isinstance(t, Tensor) else list(t)
+
+
+def _in_memory_order(t: Tensor, like: Tensor) -> Tensor:
+    """t's values in the order in which ``like`` (without gaps) holds its own."""
+    if t.stride() != like.stride():
+        t = torch.empty_strided(like.shape, like.stride(), dtype=t.dtype, device=t.device).copy_(t)
+    return torch.as_strided(t, (t.numel(),), (1,))
+
+
+@torch.no_grad()
+def adamw_step(params, grads, exp_avg: Moment, exp_avg_sq: Moment, step: Tensor, lr,
+               betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
+               seed: int = 0) -> None:
+    """The semantics of K17, in elementary fp32 operations (see ops.adamw_step)."""
+    params, grads = as_list(params), as_list(grads)
+    if not params or len(params) != len(grads):
+        raise RuntimeError("adamw_step: as many gradients as parameters are wanted")
+    numel = sum(p.numel() for p in params)
+    eight = not isinstance(exp_avg, Tensor)
+    if eight != (not isinstance(exp_avg_sq, Tensor)):
+        raise RuntimeError("adamw_step: both moments in the same bits")
+    for moment in (exp_avg, exp_avg_sq):
+        values = moment[0] if eight else moment
+        if values.numel() != numel or values.dtype != (torch.uint8 if eight else torch.float32) or (
+                eight and moment[1].numel() != -(-numel // ADAMW_BLOCK)):
+            raise RuntimeError("adamw_step: a moment must have a value for each parameter")
+    for p, g in zip(params, grads):
+        if p.shape != g.shape:
+            raise RuntimeError("adamw_step: a gradient must have its parameter's shape")
+    step += 1
+    t = int(step)
+    lr = float(lr)
+    c1 = lr / -math.expm1(t * math.log(betas[0])) if betas[0] else lr
+    c2 = 1 / math.sqrt(-math.expm1(t * math.log(betas[1]))) if betas[1] else 1.0
+    g = torch.cat([_in_memory_order(x, p) for p, x in zip(params, grads)]).float()
+    p = torch.cat([_in_memory_order(x, x) for x in params])
+    m = adamw_decode(*exp_avg, True) if eight else exp_avg
+    v = adamw_decode(*exp_avg_sq, False) if eight else exp_avg_sq
+    m = betas[0] * m + (1 - betas[0]) * g
+    v = betas[1] * v + (1 - betas[1]) * (g * g)
+    # a root in 64 bits rounds to the right one in 32, which the CPU's own need not be
+    root = v.double().sqrt().float()
+    new = p.float() * (1 - lr * weight_decay) - c1 * (m / (root * c2 + eps))
+    u_m, u_v, u_p = adamw_dither(numel, seed, t, p.device)
+    if p.dtype == torch.bfloat16:
+        bits = new.view(torch.int32).to(torch.int64) & 0xFFFFFFFF
+        up = torch.where((bits & 0x7F800000) == 0x7F800000, 0, u_p)
+        rounded = ((bits + up) >> 16) << 16
+        rounded = torch.where(rounded >= 1 << 31, rounded - (1 << 32), rounded).to(torch.int32)
+        new = torch.where(torch.isnan(new), new, rounded.view(torch.float32)).to(p.dtype)
+    for x, y in zip(params, new.split([x.numel() for x in params])):
+        torch.as_strided(x, (x.numel(),), (1,)).copy_(y)
+    if eight:
+        for state, value in zip((exp_avg, exp_avg_sq),
+                                (adamw_encode(m, True, u_m), adamw_encode(v, False, u_v))):
+            state[0].copy_(value[0])
+            state[1].copy_(value[1])
+    else:
+        exp_avg.copy_(m)
+        exp_avg_sq.copy_(v)
+
+
+# ---------------------------------------------------------------- K18
+def check_linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor],
+                     res: Optional[Tensor]) -> None:
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"linear_act: weight must be [N, K] for x [..., K], got "
+                         f"{tuple(weight.shape)} for {tuple(x.shape)}")
+    if weight.dtype != x.dtype or weight.device != x.device:
+        raise ValueError("linear_act: weight must have x's type and device")
+    n = weight.shape[0]
+    if bias is not None and (bias.shape != (n,) or bias.device != x.device
+                             or bias.dtype not in (x.dtype, torch.float32)):
+        raise ValueError(f"linear_act: bias must be [{n}] on {x.device}, {x.dtype} or fp32")
+    if res is not None and (res.shape != (*x.shape[:-1], n) or res.dtype != x.dtype
+                            or res.device != x.device):
+        raise ValueError("linear_act: res must be [..., N], of x's type and device")
+
+
+def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: str = "none",
+               res: Optional[Tensor] = None) -> Tensor:
+    """y = act(x @ weight.T + bias + res), in 32 bits and rounded once."""
+    check_linear_act(x, weight, bias, res)
+    check_act(act)
+    z = _wide(x) @ _wide(weight).t()
+    if bias is not None:
+        z = z + _wide(bias)
+    if res is not None:
+        z = z + _wide(res)
+    return _activate(z, act).to(x.dtype)
