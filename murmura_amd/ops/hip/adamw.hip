@@ -36,6 +36,7 @@ namespace {
 
 constexpr int NT = 256;
 constexpr int QB = 256;  // values that share a scale
+constexpr int MAX_BLOCKS = 256 * 8;  // as many as the CUs hold at once
 
 struct Segment {
   void* p;
@@ -49,6 +50,7 @@ constexpr int MAX_SEGMENTS = 160;
 struct Table {
   int count;
   int64_t begin, end;  // the places of this launch
+  bool last;           // the step ends with it
   Segment s[MAX_SEGMENTS];
 };
 
@@ -57,6 +59,7 @@ struct Moments {  // fp32, or codes and exponents
   void* v;
   unsigned char* me;
   unsigned char* ve;
+  bool whole;  // on 16 bytes (codes: on 8)
 };
 
 struct Hyper {
@@ -65,23 +68,24 @@ struct Hyper {
   double lr, decay;
   const float* lr_dev;  // in place of lr, where the caller keeps it on the device
   unsigned int seed;
-  const int64_t* step;  // steps done before this one
+  int64_t* step;  // steps done before this one, fewer than 2^32
 };
 
 // what is the same for all elements of a step
 struct Now {
   float keep, c1, c2;
-  unsigned int key;
+  unsigned int key, t;
 };
 
 __device__ __forceinline__ Now now_of(const Hyper& h) {
-  const int64_t t = *h.step + 1;
+  const unsigned int t = *(const unsigned int*)h.step + 1;
   const double lr = h.lr_dev ? (double)*h.lr_dev : h.lr;
   Now n;
   n.keep = (float)(1.0 - lr * h.decay);
   n.c1 = (float)(lr / -expm1((double)t * h.log_b1));
   n.c2 = (float)(1.0 / sqrt(-expm1((double)t * h.log_b2)));
-  n.key = (h.seed * 0x9E3779B1u) ^ ((unsigned int)t * 0x85A308D3u + 0x3C6EF372u);
+  n.key = (h.seed * 0x9E3779B1u) ^ (t * 0x85A308D3u + 0x3C6EF372u);
+  n.t = t;
   return n;
 }
 
@@ -106,27 +110,22 @@ __device__ __forceinline__ bf16 dithered_bf16(float f, unsigned int x) {
 template <bool FIRST>
 struct Code {
   static constexpr int TOP = FIRST ? 15 : 31;
-  static constexpr int LOW = -(TOP + 2);
   static constexpr unsigned int NAN_CODE = 8 * TOP + 7;
 
+  // A code's bits at the place of a float's: the exponent then is off by 127 - TOP, and what has no
+  // leading one is a denormal float. One ldexp puts both right, either way.
   __device__ static __forceinline__ float decode(unsigned int c, int e) {
     const unsigned int mag = FIRST ? c & 127u : c;
-    const int ex = (int)(mag >> 3);
-    const float f = (float)((mag & 7u) + (ex ? 8u : 0u));
-    float v = ldexpf(f, (ex ? ex - 1 : 0) + LOW + e - 126);
+    float v = ldexpf(__uint_as_float(mag << 20), 127 - TOP + e - 126);
     if (mag == NAN_CODE) v = __uint_as_float(0x7FC00000u);
-    return FIRST && (c & 128u) ? -v : v;
+    return FIRST ? __uint_as_float(__float_as_uint(v) | (c & 128u) << 24) : v;
   }
 
   __device__ static __forceinline__ unsigned int encode(float x, int e, unsigned int dither) {
     const unsigned int bits = __float_as_uint(x), a = bits & 0x7FFFFFFFu;
-    const float s = ldexpf(__uint_as_float(a), 126 - e);
-    unsigned int c;
-    if (s >= (FIRST ? 0x1p-14f : 0x1p-30f))
-      c = ((__float_as_uint(s) + (dither << 4) + 8u) >> 20) - 8 * (127 - TOP);
-    else
-      c = (unsigned int)(s * (FIRST ? 0x1p17f : 0x1p33f) + ((float)dither + 0.5f) * 0x1p-16f);
-    if (!FIRST && a) c = max(c, 1u);
+    const float s = ldexpf(__uint_as_float(a), 126 - e - (127 - TOP));
+    unsigned int c = (__float_as_uint(s) + (dither << 4) + 8u) >> 20;
+    if (!FIRST) c = max(c, min(a, 1u));
     if (a >= 0x7F800000u) c = NAN_CODE;
     return FIRST ? c | (bits >> 31) << 7 : c;
   }
@@ -137,96 +136,172 @@ __device__ __forceinline__ unsigned int finite_bits(float x) {
   return a < 0x7F800000u ? a : 0u;
 }
 
-// the segment that holds a place: the last that starts at or before it
+// the segment that holds a place, the last that starts at or before it: a wave looks at 64 of
+// them at once
 __device__ __forceinline__ int segment_of(const Table& t, int64_t place) {
-  int lo = 0, hi = t.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (t.s[mid].start <= place)
-      lo = mid;
-    else
-      hi = mid - 1;
-  }
-  return lo;
+  const int lane = threadIdx.x & 63;
+  int n = 0;
+  for (int base = 0; base < t.count; base += 64)
+    n += __popcll(__ballot(base + lane < t.count && t.s[base + lane].start <= place));
+  return n - 1;
 }
 
-// A thread takes 8 values in a row, 32 threads a block of 256 with one scale.
-template <typename T, typename GT, bool EIGHT>
-__global__ __launch_bounds__(NT) void adamw_kernel(Table t, Moments st, Hyper h) {
-  __shared__ Now shared_now;
-  if (threadIdx.x == 0) shared_now = now_of(h);
-  __syncthreads();
-  const Now now = shared_now;
-  const int64_t first = t.begin + ((int64_t)blockIdx.x * NT + threadIdx.x) * 8;
-  const int n = (int)max((int64_t)0, min((int64_t)8, t.end - first));
-  float p[8], g[8], m[8], v[8];
-  T* pp[8];
-  int me = 0, ve = 0;
-  if (EIGHT && n > 0) {
-    me = st.me[first / QB];
-    ve = st.ve[first / QB];
-  }
-  int seg = n > 0 ? segment_of(t, first) : 0;
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
+  constexpr int V = 16 / sizeof(T);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    m[i] = v[i] = 0.f;
-    if (i >= n) continue;
-    const int64_t place = first + i;
-    while (seg + 1 < t.count && t.s[seg + 1].start <= place) ++seg;
-    const int64_t at = place - t.s[seg].start;
-    pp[i] = (T*)t.s[seg].p + at;
-    p[i] = to_float(*pp[i]);
-    g[i] = to_float(((const GT*)t.s[seg].g)[at]);
-    if (EIGHT) {
-      m[i] = Code<true>::decode(((const unsigned char*)st.m)[place], me);
-      v[i] = Code<false>::decode(((const unsigned char*)st.v)[place], ve);
-    } else {
-      m[i] = ((const float*)st.m)[place];
-      v[i] = ((const float*)st.v)[place];
-    }
-    m[i] = h.b1 * m[i] + h.b1c * g[i];
-    v[i] = h.b2 * v[i] + h.b2c * (g[i] * g[i]);
-    p[i] = p[i] * now.keep - now.c1 * (m[i] / (sqrtf(v[i]) * now.c2 + h.eps));
+  for (int i = 0; i < 8; i += V) {
+    const Vec<T, V> v = *(const Vec<T, V>*)(p + i);
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[i + j] = to_float(v.e[j]);
   }
-  if (EIGHT) {
-    unsigned int ma = 0, va = 0;
+}
+
+// A thread takes 8 values in a row, 32 threads the 256 of one scale, a block 2048 at a time. Where
+// the 8 lie in one tensor, on 16 bytes, they are moved as a whole, else one by one; the arithmetic
+// is the same.
+template <typename T, typename GT, bool EIGHT>
+__global__ __launch_bounds__(NT) void adamw_kernel(Table t, Moments st, Hyper h, int64_t chunks) {
+  const Now now = now_of(h);
+  for (int64_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+    const int64_t first = t.begin + (chunk * NT + threadIdx.x) * 8;
+    const int n = (int)max((int64_t)0, min((int64_t)8, t.end - first));
+    int seg = t.count == 1 ? 0 : segment_of(t, t.begin + (chunk * NT + (threadIdx.x & ~63)) * 8);
+    float p[8], g[8], m[8], v[8];
+    T* pp = nullptr;
+    bool whole = false;
+    alignas(8) unsigned int cm[2], cv[2];
+    int me = 0, ve = 0;
+    if (n > 0) {
+      while (seg + 1 < t.count && t.s[seg + 1].start <= first) ++seg;
+      const int64_t at = first - t.s[seg].start;
+      pp = (T*)t.s[seg].p + at;
+      const GT* gp = (const GT*)t.s[seg].g + at;
+      whole = n == 8 && st.whole && (seg + 1 == t.count || t.s[seg + 1].start >= first + 8) &&
+              ((uintptr_t)pp | (uintptr_t)gp) % 16 == 0;
+      if (EIGHT) {
+        me = st.me[first / QB];
+        ve = st.ve[first / QB];
+      }
+      if (whole) {
+        load8(pp, p);
+        load8(gp, g);
+        if (EIGHT) {
+          *(uint2*)cm = *(const uint2*)((const unsigned char*)st.m + first);
+          *(uint2*)cv = *(const uint2*)((const unsigned char*)st.v + first);
+        } else {
+          load8((const float*)st.m + first, m);
+          load8((const float*)st.v + first, v);
+        }
+      } else {
+        cm[0] = cm[1] = cv[0] = cv[1] = 0;
+        int sg = seg;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (i >= n) continue;
+          while (sg + 1 < t.count && t.s[sg + 1].start <= first + i) ++sg;
+          const int64_t place = first + i - t.s[sg].start;
+          p[i] = to_float(((const T*)t.s[sg].p)[place]);
+          g[i] = to_float(((const GT*)t.s[sg].g)[place]);
+          if (EIGHT) {
+            cm[i / 4] |= (unsigned int)((const unsigned char*)st.m)[first + i] << (i % 4 * 8);
+            cv[i / 4] |= (unsigned int)((const unsigned char*)st.v)[first + i] << (i % 4 * 8);
+          } else {
+            m[i] = ((const float*)st.m)[first + i];
+            v[i] = ((const float*)st.v)[first + i];
+          }
+        }
+      }
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      ma = max(ma, finite_bits(m[i]));
-      va = max(va, finite_bits(v[i]));
+      if (i >= n) {
+        m[i] = v[i] = p[i] = 0.f;
+        continue;
+      }
+      if (EIGHT) {
+        m[i] = Code<true>::decode(cm[i / 4] >> (i % 4 * 8) & 255u, me);
+        v[i] = Code<false>::decode(cv[i / 4] >> (i % 4 * 8) & 255u, ve);
+      }
+      m[i] = h.b1 * m[i] + h.b1c * g[i];
+      v[i] = h.b2 * v[i] + h.b2c * (g[i] * g[i]);
+      p[i] = p[i] * now.keep - now.c1 * (m[i] / (sqrtf(v[i]) * now.c2 + h.eps));
     }
+    if (EIGHT) {
+      unsigned int ma = 0, va = 0;
 #pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      ma = max(ma, (unsigned int)__shfl_xor((int)ma, off, 64));
-      va = max(va, (unsigned int)__shfl_xor((int)va, off, 64));
+      for (int i = 0; i < 8; ++i) {
+        ma = max(ma, finite_bits(m[i]));
+        va = max(va, finite_bits(v[i]));
+      }
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        ma = max(ma, (unsigned int)__shfl_xor((int)ma, off, 64));
+        va = max(va, (unsigned int)__shfl_xor((int)va, off, 64));
+      }
+      me = (int)(ma >> 23);
+      ve = (int)(va >> 23);
     }
-    me = (int)(ma >> 23);
-    ve = (int)(va >> 23);
-    if (n > 0 && (threadIdx.x & 31) == 0) {
+    if (n == 0) continue;
+    if (EIGHT && (threadIdx.x & 31) == 0) {
       st.me[first / QB] = (unsigned char)me;
       st.ve[first / QB] = (unsigned char)ve;
     }
-  }
+    alignas(16) T q[8];
+    cm[0] = cm[1] = cv[0] = cv[1] = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (i >= n) continue;
-    const int64_t place = first + i;
-    const unsigned int x = hash_of((unsigned int)place, now.key);
-    if constexpr (sizeof(T) == 2)
-      *pp[i] = dithered_bf16(p[i], x);
-    else
-      *pp[i] = p[i];
-    if (EIGHT) {
-      ((unsigned char*)st.m)[place] = (unsigned char)Code<true>::encode(m[i], me, x & 0xFFFFu);
-      ((unsigned char*)st.v)[place] = (unsigned char)Code<false>::encode(v[i], ve, x >> 16);
+    for (int i = 0; i < 8; ++i) {
+      unsigned int x = 0;
+      if (EIGHT || sizeof(T) == 2) x = hash_of((unsigned int)first + i, now.key);
+      if constexpr (sizeof(T) == 2)
+        q[i] = dithered_bf16(p[i], x);
+      else
+        q[i] = p[i];
+      if (EIGHT) {
+        cm[i / 4] |= Code<true>::encode(m[i], me, x & 0xFFFFu) << (i % 4 * 8);
+        cv[i / 4] |= Code<false>::encode(v[i], ve, x >> 16) << (i % 4 * 8);
+      }
+    }
+    if (whole) {
+      constexpr int V = 16 / sizeof(T);
+#pragma unroll
+      for (int i = 0; i < 8; i += V) *(Vec<T, V>*)(pp + i) = *(const Vec<T, V>*)(q + i);
+      if (EIGHT) {
+        *(uint2*)((unsigned char*)st.m + first) = *(const uint2*)cm;
+        *(uint2*)((unsigned char*)st.v + first) = *(const uint2*)cv;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; i += 4) {
+          *(float4*)((float*)st.m + first + i) = make_float4(m[i], m[i + 1], m[i + 2], m[i + 3]);
+          *(float4*)((float*)st.v + first + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        }
+      }
     } else {
-      ((float*)st.m)[place] = m[i];
-      ((float*)st.v)[place] = v[i];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i >= n) continue;
+        while (seg + 1 < t.count && t.s[seg + 1].start <= first + i) ++seg;
+        ((T*)t.s[seg].p)[first + i - t.s[seg].start] = q[i];
+        if (EIGHT) {
+          ((unsigned char*)st.m)[first + i] = (unsigned char)(cm[i / 4] >> (i % 4 * 8));
+          ((unsigned char*)st.v)[first + i] = (unsigned char)(cv[i / 4] >> (i % 4 * 8));
+        } else {
+          ((float*)st.m)[first + i] = m[i];
+          ((float*)st.v)[first + i] = v[i];
+        }
+      }
     }
   }
+  // The block that ends last counts the step. The high half of the count tells how many blocks of
+  // the last launch have read it, and is zero again when the launch ends.
+  if (!t.last) return;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    unsigned int* halves = (unsigned int*)h.step;
+    if (atomicAdd(halves + 1, 1u) == gridDim.x - 1)
+      atomicExch((unsigned long long*)h.step, (unsigned long long)(now.t));
+  }
 }
-
-__global__ void adamw_count_kernel(int64_t* step) { *step += 1; }
 
 template <typename O, bool FIRST>
 __global__ __launch_bounds__(NT) void adamw_decode_kernel(const unsigned char* __restrict__ c,
@@ -296,7 +371,8 @@ void adamw_step(const std::vector<Tensor>& params, std::vector<Tensor> grads,
                 "adamw_step: lr on the device is one fp32 value");
   const hipStream_t st = stream_of(step);
   const bool eight = exp_avg.size() == 2;
-  Moments mo{exp_avg[0].data_ptr(), exp_avg_sq[0].data_ptr(), nullptr, nullptr};
+  Moments mo{exp_avg[0].data_ptr(), exp_avg_sq[0].data_ptr(), nullptr, nullptr, false};
+  mo.whole = ((uintptr_t)mo.m | (uintptr_t)mo.v) % (eight ? 8 : 16) == 0;
   if (eight) {
     mo.me = (unsigned char*)exp_avg[1].data_ptr();
     mo.ve = (unsigned char*)exp_avg_sq[1].data_ptr();
@@ -332,15 +408,16 @@ void adamw_step(const std::vector<Tensor>& params, std::vector<Tensor> grads,
     t.end = i == params.size() ? P : eight ? at / QB * QB : at;
     TORCH_CHECK(t.end > t.begin, "adamw_step: over ", MAX_SEGMENTS, " tensors within ", QB,
                 " values of 8-bit moments: pass them as one");
-    const int64_t blocks = ceil_div(t.end - t.begin, (int64_t)NT * 8);
-    TORCH_CHECK(blocks < (1LL << 31), "adamw_step: too many values");
+    t.last = t.end == P;
+    const int64_t chunks = ceil_div(t.end - t.begin, (int64_t)NT * 8);
+    const int64_t blocks = std::min<int64_t>(chunks, MAX_BLOCKS);
     MM_DISPATCH_TYPE(params[0], {
       if (gtype == type) {
-        if (eight) adamw_kernel<T, T, true><<<(unsigned)blocks, NT, 0, st>>>(t, mo, h);
-        else adamw_kernel<T, T, false><<<(unsigned)blocks, NT, 0, st>>>(t, mo, h);
+        if (eight) adamw_kernel<T, T, true><<<(unsigned)blocks, NT, 0, st>>>(t, mo, h, chunks);
+        else adamw_kernel<T, T, false><<<(unsigned)blocks, NT, 0, st>>>(t, mo, h, chunks);
       } else {
-        if (eight) adamw_kernel<T, float, true><<<(unsigned)blocks, NT, 0, st>>>(t, mo, h);
-        else adamw_kernel<T, float, false><<<(unsigned)blocks, NT, 0, st>>>(t, mo, h);
+        if (eight) adamw_kernel<T, float, true><<<(unsigned)blocks, NT, 0, st>>>(t, mo, h, chunks);
+        else adamw_kernel<T, float, false><<<(unsigned)blocks, NT, 0, st>>>(t, mo, h, chunks);
       }
     });
     check_launch("adamw_step");
@@ -348,8 +425,7 @@ void adamw_step(const std::vector<Tensor>& params, std::vector<Tensor> grads,
     while (next < i && start + params[next].numel() <= t.end) start += params[next++].numel();
     t.begin = t.end;
   }
-  adamw_count_kernel<<<1, 1, 0, st>>>(step.data_ptr<int64_t>());
-  check_launch("adamw_step");
+  if (P == 0) step.add_(1);
 }
 
 Tensor adamw_decode(const Tensor& codes, const Tensor& exps, bool first, bool half) {

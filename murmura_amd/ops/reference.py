@@ -287,16 +287,16 @@ def adamw_decode(codes: Tensor, exps: Tensor, first: bool) -> Tensor:
 
 def adamw_encode(x: Tensor, first: bool, dither: Tensor) -> Tuple[Tensor, Tensor]:
     """(codes, exponents) of fp32 values [P]; dither: 16 random bits a value."""
-    top, least = _moment_form(first)
+    top = _moment_form(first)[0]
     a = x.abs()
     finite = torch.isfinite(x)
     blocks = torch.nn.functional.pad(a.masked_fill(~finite, 0.0), (0, -x.numel() % ADAMW_BLOCK))
     exps = blocks.view(-1, ADAMW_BLOCK).amax(1).view(torch.int32) >> 23
-    scale = _pow2(exps - 126).repeat_interleave(ADAMW_BLOCK)[: x.numel()]
-    s = (a.double() / scale).float()
-    whole = ((s.view(torch.int32).to(torch.int64) + (dither << 4) + 8) >> 20) - 8 * (127 - top)
-    small = (s / least + (dither.float() + 0.5) / 65536).floor().nan_to_num(0.0).clamp(0, 255)
-    code = torch.where(s >= 8 * least, whole, small.to(torch.int64))
+    # the code's bits are the top bits of a float whose exponent is off by 127 - top; without a
+    # leading one, of a denormal float
+    shift = _pow2(top - 1 - exps).repeat_interleave(ADAMW_BLOCK)[: x.numel()]
+    bits = (a.double() * shift).float().view(torch.int32).to(torch.int64)
+    code = (bits + (dither << 4) + 8) >> 20
     if not first:
         code = torch.where(a > 0, code.clamp_min(1), code)
     code = torch.where(finite, code, 8 * top + 7)
