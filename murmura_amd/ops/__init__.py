@@ -292,9 +292,7 @@ def adamw_dequantize(exp_avg: ref.Moment, exp_avg_sq: ref.Moment,
     if dtype not in (torch.float32, torch.bfloat16):
         raise ValueError(f"adamw_dequantize: fp32 or bf16, not {dtype}")
     if _use_native(exp_avg[0]):
-        half = dtype == torch.bfloat16
-        return (_EXT.adamw_decode(exp_avg[0], exp_avg[1], True, half),
-                _EXT.adamw_decode(exp_avg_sq[0], exp_avg_sq[1], False, half))
+        return _EXT.adamw_decode(list(exp_avg), list(exp_avg_sq), dtype == torch.bfloat16)
     return (ref.adamw_decode(*exp_avg, True).to(dtype), ref.adamw_decode(*exp_avg_sq, False).to(dtype))
 
 

@@ -23,7 +23,8 @@
 // hash of (seed, step, place), so a run repeats bit for bit.
 //
 // Every operation is rounded by itself (no contraction): an element's result
-// does not depend on which path, vector width or compiler it went through.
+// does not depend on which path, vector width or compiler it went through, and
+// the moments are those of elementary fp32 operations bit for bit.
 
 #include "kernel_common.h"
 
@@ -113,28 +114,32 @@ struct Code {
   static constexpr unsigned int NAN_CODE = 8 * TOP + 7;
 
   // A code's bits at the place of a float's: the exponent then is off by 127 - TOP, and what has no
-  // leading one is a denormal float. One ldexp puts both right, either way.
+  // leading one is a denormal float. One ldexp puts both right, either way. What is not finite is
+  // looked for in several values at once (odd_codes, the largest bits) and put right apart.
   __device__ static __forceinline__ float decode(unsigned int c, int e) {
-    const unsigned int mag = FIRST ? c & 127u : c;
-    float v = ldexpf(__uint_as_float(mag << 20), 127 - TOP + e - 126);
-    if (mag == NAN_CODE) v = __uint_as_float(0x7FC00000u);
+    const float v = ldexpf(__uint_as_float((FIRST ? c & 127u : c) << 20), 127 - TOP + e - 126);
     return FIRST ? __uint_as_float(__float_as_uint(v) | (c & 128u) << 24) : v;
   }
-
+  __device__ static __forceinline__ bool is_nan(unsigned int c) {
+    return (FIRST ? c & 127u : c) == NAN_CODE;
+  }
+  // whether one of four codes is a NaN (or, seldom, the code after one): a byte without its
+  // complement is zero
+  __device__ static __forceinline__ bool odd_codes(unsigned int c4) {
+    const unsigned int x = FIRST ? ~c4 & 0x7F7F7F7Fu : ~c4;
+    return ((x - 0x01010101u) & ~x & 0x80808080u) != 0;
+  }
   __device__ static __forceinline__ unsigned int encode(float x, int e, unsigned int dither) {
     const unsigned int bits = __float_as_uint(x), a = bits & 0x7FFFFFFFu;
     const float s = ldexpf(__uint_as_float(a), 126 - e - (127 - TOP));
-    unsigned int c = (__float_as_uint(s) + (dither << 4) + 8u) >> 20;
+    unsigned int c = (__float_as_uint(s) + (dither << 4 | 8u)) >> 20;
     if (!FIRST) c = max(c, min(a, 1u));
-    if (a >= 0x7F800000u) c = NAN_CODE;
     return FIRST ? c | (bits >> 31) << 7 : c;
   }
 };
 
-__device__ __forceinline__ unsigned int finite_bits(float x) {
-  const unsigned int a = __float_as_uint(x) & 0x7FFFFFFFu;
-  return a < 0x7F800000u ? a : 0u;
-}
+constexpr unsigned int INF_BITS = 0x7F800000u;
+__device__ __forceinline__ unsigned int abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
 
 // the segment that holds a place, the last that starts at or before it: a wave looks at 64 of
 // them at once
@@ -198,6 +203,7 @@ __global__ __launch_bounds__(NT) void adamw_kernel(Table t, Moments st, Hyper h,
         int sg = seg;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
+          p[i] = g[i] = m[i] = v[i] = 0.f;
           if (i >= n) continue;
           while (sg + 1 < t.count && t.s[sg + 1].start <= first + i) ++sg;
           const int64_t place = first + i - t.s[sg].start;
@@ -213,26 +219,51 @@ __global__ __launch_bounds__(NT) void adamw_kernel(Table t, Moments st, Hyper h,
         }
       }
     }
+    if (n == 0) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (i >= n) {
-        m[i] = v[i] = p[i] = 0.f;
-        continue;
-      }
-      if (EIGHT) {
+      for (int i = 0; i < 8; ++i) m[i] = v[i] = p[i] = g[i] = 0.f;
+      cm[0] = cm[1] = cv[0] = cv[1] = 0;
+    }
+    if (EIGHT) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
         m[i] = Code<true>::decode(cm[i / 4] >> (i % 4 * 8) & 255u, me);
         v[i] = Code<false>::decode(cv[i / 4] >> (i % 4 * 8) & 255u, ve);
       }
+      if (Code<true>::odd_codes(cm[0]) || Code<true>::odd_codes(cm[1]) ||
+          Code<false>::odd_codes(cv[0]) || Code<false>::odd_codes(cv[1])) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (Code<true>::is_nan(cm[i / 4] >> (i % 4 * 8) & 255u)) m[i] = __uint_as_float(0x7FC00000u);
+          if (Code<false>::is_nan(cv[i / 4] >> (i % 4 * 8) & 255u)) v[i] = __uint_as_float(0x7FC00000u);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
       m[i] = h.b1 * m[i] + h.b1c * g[i];
       v[i] = h.b2 * v[i] + h.b2c * (g[i] * g[i]);
-      p[i] = p[i] * now.keep - now.c1 * (m[i] / (sqrtf(v[i]) * now.c2 + h.eps));
+      // root and reciprocal are within one unit in the last place: a step of 1e-3 of a parameter
+      // needs no more, and the exact ones took a quarter of all instructions
+      const float root = __builtin_amdgcn_sqrtf(v[i]);
+      p[i] = p[i] * now.keep - now.c1 * (m[i] * __builtin_amdgcn_rcpf(root * now.c2 + h.eps));
     }
+    bool odd = false;
     if (EIGHT) {
       unsigned int ma = 0, va = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        ma = max(ma, finite_bits(m[i]));
-        va = max(va, finite_bits(v[i]));
+        ma = max(ma, abs_bits(m[i]));
+        va = max(va, abs_bits(v[i]));
+      }
+      odd = max(ma, va) >= INF_BITS;
+      if (odd) {  // the largest of what is finite
+        ma = va = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          ma = max(ma, abs_bits(m[i]) < INF_BITS ? abs_bits(m[i]) : 0u);
+          va = max(va, abs_bits(v[i]) < INF_BITS ? abs_bits(v[i]) : 0u);
+        }
       }
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
@@ -258,8 +289,15 @@ __global__ __launch_bounds__(NT) void adamw_kernel(Table t, Moments st, Hyper h,
       else
         q[i] = p[i];
       if (EIGHT) {
-        cm[i / 4] |= Code<true>::encode(m[i], me, x & 0xFFFFu) << (i % 4 * 8);
-        cv[i / 4] |= Code<false>::encode(v[i], ve, x >> 16) << (i % 4 * 8);
+        cm[i / 4] |= (Code<true>::encode(m[i], me, x & 0xFFFFu) & 255u) << (i % 4 * 8);
+        cv[i / 4] |= (Code<false>::encode(v[i], ve, x >> 16) & 255u) << (i % 4 * 8);
+      }
+    }
+    if (EIGHT && odd) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {  // sign of m aside, all bits
+        if (abs_bits(m[i]) >= INF_BITS) cm[i / 4] |= Code<true>::NAN_CODE << (i % 4 * 8);
+        if (abs_bits(v[i]) >= INF_BITS) cv[i / 4] |= Code<false>::NAN_CODE << (i % 4 * 8);
       }
     }
     if (whole) {
@@ -303,15 +341,39 @@ __global__ __launch_bounds__(NT) void adamw_kernel(Table t, Moments st, Hyper h,
   }
 }
 
+// Both moments' values, 8 a thread.
 template <typename O, bool FIRST>
-__global__ __launch_bounds__(NT) void adamw_decode_kernel(const unsigned char* __restrict__ c,
-                                                          const unsigned char* __restrict__ e,
-                                                          int64_t P, O* __restrict__ out) {
-  const int64_t first = ((int64_t)blockIdx.x * NT + threadIdx.x) * 8;
+__device__ __forceinline__ void decode8(const unsigned char* __restrict__ c,
+                                        const unsigned char* __restrict__ e, int64_t first, int64_t P,
+                                        bool whole, O* __restrict__ out) {
+  const int ex = e[first / QB];
+  alignas(8) unsigned char in[8] = {};
+  alignas(16) O o[8];
+  const int n = (int)min((int64_t)8, P - first);
+  if (whole && n == 8)
+    *(uint2*)in = *(const uint2*)(c + first);
+  else
+    for (int i = 0; i < n; ++i) in[i] = c[first + i];
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    if (first + i < P)
-      out[first + i] = from_float<O>(Code<FIRST>::decode(c[first + i], e[first / QB]));
+    o[i] = from_float<O>(Code<FIRST>::is_nan(in[i]) ? __uint_as_float(0x7FC00000u)
+                                                    : Code<FIRST>::decode(in[i], ex));
+  if (n == 8) {
+    constexpr int V = 16 / sizeof(O);
+#pragma unroll
+    for (int i = 0; i < 8; i += V) *(Vec<O, V>*)(out + first + i) = *(const Vec<O, V>*)(o + i);
+  } else {
+    for (int i = 0; i < n; ++i) out[first + i] = o[i];
+  }
+}
+
+template <typename O>
+__global__ __launch_bounds__(NT) void adamw_decode_kernel(Moments st, int64_t P, O* __restrict__ m,
+                                                          O* __restrict__ v) {
+  const int64_t first = ((int64_t)blockIdx.x * NT + threadIdx.x) * 8;
+  if (first >= P) return;
+  decode8<O, true>((const unsigned char*)st.m, st.me, first, P, st.whole, m);
+  decode8<O, false>((const unsigned char*)st.v, st.ve, first, P, st.whole, v);
 }
 
 void check_state(const std::vector<Tensor>& s, int64_t P, const at::Device& d) {
@@ -428,26 +490,28 @@ void adamw_step(const std::vector<Tensor>& params, std::vector<Tensor> grads,
   if (P == 0) step.add_(1);
 }
 
-Tensor adamw_decode(const Tensor& codes, const Tensor& exps, bool first, bool half) {
-  TORCH_CHECK(codes.is_cuda() && codes.scalar_type() == at::kByte && codes.is_contiguous() &&
-                  exps.scalar_type() == at::kByte && exps.is_contiguous() &&
-                  exps.device() == codes.device() && exps.numel() == ceil_div(codes.numel(), QB),
-              "adamw_dequantize: codes [P] and exponents [ceil(P/256)], uint8");
-  const c10::DeviceGuard guard(codes.device());
-  Tensor out = at::empty(codes.sizes(), codes.options().dtype(half ? at::kBFloat16 : at::kFloat));
-  const int64_t P = codes.numel();
-  if (P == 0) return out;
+std::tuple<Tensor, Tensor> adamw_decode(const std::vector<Tensor>& exp_avg,
+                                        const std::vector<Tensor>& exp_avg_sq, bool half) {
+  TORCH_CHECK(exp_avg.size() == 2 && exp_avg_sq.size() == 2 && exp_avg[0].is_cuda(),
+              "adamw_dequantize: 8-bit moments on a GPU are wanted");
+  const int64_t P = exp_avg[0].numel();
+  check_state(exp_avg, P, exp_avg[0].device());
+  check_state(exp_avg_sq, P, exp_avg[0].device());
+  const c10::DeviceGuard guard(exp_avg[0].device());
+  const auto options = exp_avg[0].options().dtype(half ? at::kBFloat16 : at::kFloat);
+  Tensor m = at::empty({P}, options), v = at::empty({P}, options);
+  if (P == 0) return {m, v};
   const int64_t blocks = ceil_div(P, (int64_t)NT * 8);
   TORCH_CHECK(blocks < (1LL << 31), "adamw_dequantize: too many values");
-  const hipStream_t st = stream_of(codes);
-  const auto* c = (const unsigned char*)codes.data_ptr();
-  const auto* e = (const unsigned char*)exps.data_ptr();
-  MM_DISPATCH_TYPE(out, {
-    if (first) adamw_decode_kernel<T, true><<<(unsigned)blocks, NT, 0, st>>>(c, e, P, (T*)out.data_ptr());
-    else adamw_decode_kernel<T, false><<<(unsigned)blocks, NT, 0, st>>>(c, e, P, (T*)out.data_ptr());
+  Moments mo{exp_avg[0].data_ptr(), exp_avg_sq[0].data_ptr(), (unsigned char*)exp_avg[1].data_ptr(),
+             (unsigned char*)exp_avg_sq[1].data_ptr(), false};
+  mo.whole = ((uintptr_t)mo.m | (uintptr_t)mo.v) % 8 == 0;
+  MM_DISPATCH_TYPE(m, {
+    adamw_decode_kernel<T><<<(unsigned)blocks, NT, 0, stream_of(m)>>>(mo, P, (T*)m.data_ptr(),
+                                                                      (T*)v.data_ptr());
   });
   check_launch("adamw_dequantize");
-  return out;
+  return {m, v};
 }
 
 }  // namespace
@@ -457,8 +521,8 @@ void bind_adamw(pybind11::module_& m) {
         py::arg("params"), py::arg("grads"), py::arg("exp_avg"), py::arg("exp_avg_sq"),
         py::arg("step"), py::arg("lr"), py::arg("lr_tensor"), py::arg("b1"), py::arg("b2"),
         py::arg("eps"), py::arg("decay"), py::arg("seed"));
-  m.def("adamw_decode", &adamw_decode, "K17: the values of an 8-bit moment", py::arg("codes"),
-        py::arg("exps"), py::arg("first"), py::arg("half"));
+  m.def("adamw_decode", &adamw_decode, "K17: the values of 8-bit moments", py::arg("exp_avg"),
+        py::arg("exp_avg_sq"), py::arg("half"));
 }
 
 }  // namespace mm

@@ -353,7 +353,12 @@ ADAMW_SHAPES = [
 @pytest.mark.parametrize("bits", [8, 32])
 @pytest.mark.parametrize("shapes", ADAMW_SHAPES, ids=lambda s: f"{len(s)}x{s[0]}")
 def test_adamw_step(shapes, bits, dtype, gtype):
-    """Every operation is one rounding in both, so the bits are the same."""
+    """Moments: every operation is one rounding in both, so the bits are the
+    same. Parameters: root and reciprocal are off by a unit (2 U) each, which
+    with the roundings of three products stays below 8 U of the step (|m| <= 3.2
+    sqrt(v) after so few steps, so a step is at most 5 lr); two sums round to U
+    of a parameter below 1. In bf16 a value so near a border may go to the other
+    side: 2^-8 of itself."""
     if bits == 8 and len(shapes) == 400:
         pytest.skip("refused: see test_adamw_refusals")
     cpu = _adamw_case(shapes, dtype, bits, 3, "cpu", gtype)
@@ -361,7 +366,14 @@ def test_adamw_step(shapes, bits, dtype, gtype):
     for k in range(3):
         for _, params, grads, state in (cpu, gpu):
             ops.adamw_step(params, [g * (k + 1) for g in grads], *state, 1e-2, weight_decay=0.1, seed=k * 977 - 5)
-    assert torch.equal(cpu[0], gpu[0].cpu())
+    tol = 3 * (8 * U * 5 * 1e-2 + 2 * U)
+    diff = (cpu[0].double() - gpu[0].cpu().double()).abs()
+    if dtype == FP32:
+        assert diff.max() <= tol
+    else:
+        assert (diff <= tol + 3 * 2.0 ** -8 * cpu[0].double().abs()).all()
+        # the share of values within 24 U * 0.05 of a border that lie 2^-9 * 2^-5 apart at the least
+        assert (diff > 0).sum() <= 3 + 0.01 * diff.numel()
     for a, b in zip(cpu[3][:2], gpu[3][:2]):
         for x, y in zip(_flat_state(a), _flat_state(b)):
             assert torch.equal(x, y.cpu())
