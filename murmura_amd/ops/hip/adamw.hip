@@ -97,16 +97,6 @@ __device__ __forceinline__ unsigned int hash_of(unsigned int place, unsigned int
   return x ^ (x >> 16);
 }
 
-__device__ __forceinline__ bf16 dithered_bf16(float f, unsigned int x) {
-  const unsigned int u = __float_as_uint(f);
-  bf16 r;
-  if ((u & 0x7F800000u) == 0x7F800000u)
-    r = round_bf16(f);  // an infinity or a NaN stays what it is
-  else
-    r.v = (unsigned short)((u + ((x * 0xA54FF53Bu) >> 16)) >> 16);
-  return r;
-}
-
 // FIRST: sign + 4 + 3 bits, TOP 15; else 5 + 3 bits, TOP 31
 template <bool FIRST>
 struct Code {
@@ -138,17 +128,30 @@ struct Code {
   }
 };
 
+// Keeps the compiler from working a seldom branch out for everybody.
+#define MM_SELDOM() asm volatile("")
+
 constexpr unsigned int INF_BITS = 0x7F800000u;
 __device__ __forceinline__ unsigned int abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
 
 // the segment that holds a place, the last that starts at or before it: a wave looks at 64 of
 // them at once
-__device__ __forceinline__ int segment_of(const Table& t, int64_t place) {
+__device__ __forceinline__ int segment_of(const Segment* s, int count, int64_t place) {
   const int lane = threadIdx.x & 63;
   int n = 0;
-  for (int base = 0; base < t.count; base += 64)
-    n += __popcll(__ballot(base + lane < t.count && t.s[base + lane].start <= place));
+  for (int base = 0; base < count; base += 64)
+    n += __popcll(__ballot(base + lane < count && s[base + lane].start <= place));
   return n - 1;
+}
+
+// the largest of 32 lanes, in all of them: within quads, halves and rows of 16 by the adder's own
+// lane moves, across the two rows through LDS
+__device__ __forceinline__ unsigned int max32(unsigned int x) {
+  x = max(x, (unsigned int)__builtin_amdgcn_mov_dpp((int)x, 0xB1, 0xF, 0xF, true));   // 1 0 3 2
+  x = max(x, (unsigned int)__builtin_amdgcn_mov_dpp((int)x, 0x4E, 0xF, 0xF, true));   // 2 3 0 1
+  x = max(x, (unsigned int)__builtin_amdgcn_mov_dpp((int)x, 0x141, 0xF, 0xF, true));  // half mirror
+  x = max(x, (unsigned int)__builtin_amdgcn_mov_dpp((int)x, 0x140, 0xF, 0xF, true));  // mirror
+  return max(x, (unsigned int)__shfl_xor((int)x, 16, 64));
 }
 
 template <typename T>
@@ -167,22 +170,26 @@ __device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
 // is the same.
 template <typename T, typename GT, bool EIGHT>
 __global__ __launch_bounds__(NT) void adamw_kernel(Table t, Moments st, Hyper h, int64_t chunks) {
+  // the table in LDS: a lane's look into the launch's arguments goes out to the host's memory
+  __shared__ Segment segs[MAX_SEGMENTS];
+  for (int i = threadIdx.x; i < t.count; i += NT) segs[i] = t.s[i];
   const Now now = now_of(h);
+  __syncthreads();
   for (int64_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
     const int64_t first = t.begin + (chunk * NT + threadIdx.x) * 8;
     const int n = (int)max((int64_t)0, min((int64_t)8, t.end - first));
-    int seg = t.count == 1 ? 0 : segment_of(t, t.begin + (chunk * NT + (threadIdx.x & ~63)) * 8);
+    int seg = t.count == 1 ? 0 : segment_of(segs, t.count, t.begin + (chunk * NT + (threadIdx.x & ~63)) * 8);
     float p[8], g[8], m[8], v[8];
     T* pp = nullptr;
     bool whole = false;
     alignas(8) unsigned int cm[2], cv[2];
     int me = 0, ve = 0;
     if (n > 0) {
-      while (seg + 1 < t.count && t.s[seg + 1].start <= first) ++seg;
-      const int64_t at = first - t.s[seg].start;
-      pp = (T*)t.s[seg].p + at;
-      const GT* gp = (const GT*)t.s[seg].g + at;
-      whole = n == 8 && st.whole && (seg + 1 == t.count || t.s[seg + 1].start >= first + 8) &&
+      while (seg + 1 < t.count && segs[seg + 1].start <= first) ++seg;
+      const int64_t at = first - segs[seg].start;
+      pp = (T*)segs[seg].p + at;
+      const GT* gp = (const GT*)segs[seg].g + at;
+      whole = n == 8 && st.whole && (seg + 1 == t.count || segs[seg + 1].start >= first + 8) &&
               ((uintptr_t)pp | (uintptr_t)gp) % 16 == 0;
       if (EIGHT) {
         me = st.me[first / QB];
@@ -205,10 +212,10 @@ __global__ __launch_bounds__(NT) void adamw_kernel(Table t, Moments st, Hyper h,
         for (int i = 0; i < 8; ++i) {
           p[i] = g[i] = m[i] = v[i] = 0.f;
           if (i >= n) continue;
-          while (sg + 1 < t.count && t.s[sg + 1].start <= first + i) ++sg;
-          const int64_t place = first + i - t.s[sg].start;
-          p[i] = to_float(((const T*)t.s[sg].p)[place]);
-          g[i] = to_float(((const GT*)t.s[sg].g)[place]);
+          while (sg + 1 < t.count && segs[sg + 1].start <= first + i) ++sg;
+          const int64_t place = first + i - segs[sg].start;
+          p[i] = to_float(((const T*)segs[sg].p)[place]);
+          g[i] = to_float(((const GT*)segs[sg].g)[place]);
           if (EIGHT) {
             cm[i / 4] |= (unsigned int)((const unsigned char*)st.m)[first + i] << (i % 4 * 8);
             cv[i / 4] |= (unsigned int)((const unsigned char*)st.v)[first + i] << (i % 4 * 8);
@@ -232,6 +239,7 @@ __global__ __launch_bounds__(NT) void adamw_kernel(Table t, Moments st, Hyper h,
       }
       if (Code<true>::odd_codes(cm[0]) || Code<true>::odd_codes(cm[1]) ||
           Code<false>::odd_codes(cv[0]) || Code<false>::odd_codes(cv[1])) {
+        MM_SELDOM();
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           if (Code<true>::is_nan(cm[i / 4] >> (i % 4 * 8) & 255u)) m[i] = __uint_as_float(0x7FC00000u);
@@ -258,6 +266,7 @@ __global__ __launch_bounds__(NT) void adamw_kernel(Table t, Moments st, Hyper h,
       }
       odd = max(ma, va) >= INF_BITS;
       if (odd) {  // the largest of what is finite
+        MM_SELDOM();
         ma = va = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -265,39 +274,51 @@ __global__ __launch_bounds__(NT) void adamw_kernel(Table t, Moments st, Hyper h,
           va = max(va, abs_bits(v[i]) < INF_BITS ? abs_bits(v[i]) : 0u);
         }
       }
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        ma = max(ma, (unsigned int)__shfl_xor((int)ma, off, 64));
-        va = max(va, (unsigned int)__shfl_xor((int)va, off, 64));
-      }
-      me = (int)(ma >> 23);
-      ve = (int)(va >> 23);
+      me = (int)(max32(ma) >> 23);
+      ve = (int)(max32(va) >> 23);
     }
     if (n == 0) continue;
     if (EIGHT && (threadIdx.x & 31) == 0) {
       st.me[first / QB] = (unsigned char)me;
       st.ve[first / QB] = (unsigned char)ve;
     }
+    // The codes, and the parameters in bf16: what the dither carries into stays. Values that are not
+    // finite are taken along and put right afterwards.
     alignas(16) T q[8];
+    unsigned int most = 0, cut = 0;
     cm[0] = cm[1] = cv[0] = cv[1] = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      unsigned int x = 0;
-      if (EIGHT || sizeof(T) == 2) x = hash_of((unsigned int)first + i, now.key);
-      if constexpr (sizeof(T) == 2)
-        q[i] = dithered_bf16(p[i], x);
-      else
+      if (EIGHT || sizeof(T) == 2) cut = hash_of((unsigned int)first + i, now.key);
+      if constexpr (sizeof(T) == 2) {
+        most = max(most, abs_bits(p[i]));
+        q[i].v = (unsigned short)((__float_as_uint(p[i]) + (cut * 0xA54FF53Bu >> 16)) >> 16);
+      } else {
         q[i] = p[i];
+      }
       if (EIGHT) {
-        cm[i / 4] |= (Code<true>::encode(m[i], me, x & 0xFFFFu) & 255u) << (i % 4 * 8);
-        cv[i / 4] |= (Code<false>::encode(v[i], ve, x >> 16) & 255u) << (i % 4 * 8);
+        cm[i / 4] |= Code<true>::encode(m[i], me, cut & 0xFFFFu) << (i % 4 * 8);
+        cv[i / 4] |= Code<false>::encode(v[i], ve, cut >> 16) << (i % 4 * 8);
       }
     }
     if (EIGHT && odd) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {  // sign of m aside, all bits
-        if (abs_bits(m[i]) >= INF_BITS) cm[i / 4] |= Code<true>::NAN_CODE << (i % 4 * 8);
-        if (abs_bits(v[i]) >= INF_BITS) cv[i / 4] |= Code<false>::NAN_CODE << (i % 4 * 8);
+      MM_SELDOM();
+      cm[0] = cm[1] = cv[0] = cv[1] = 0;
+      for (int i = 0; i < 8; ++i) {
+        const unsigned int x = hash_of((unsigned int)first + i, now.key);
+        const unsigned int a = abs_bits(m[i]) < INF_BITS ? Code<true>::encode(m[i], me, x & 0xFFFFu)
+                                                         : Code<true>::NAN_CODE;
+        const unsigned int b = abs_bits(v[i]) < INF_BITS ? Code<false>::encode(v[i], ve, x >> 16)
+                                                         : Code<false>::NAN_CODE;
+        cm[i / 4] |= (a | __float_as_uint(m[i]) >> 31 << 7) << (i % 4 * 8);
+        cv[i / 4] |= b << (i % 4 * 8);
+      }
+    }
+    if constexpr (sizeof(T) == 2) {
+      if (most >= INF_BITS) {
+        MM_SELDOM();
+        for (int i = 0; i < 8; ++i)
+          if (abs_bits(p[i]) >= INF_BITS) q[i] = round_bf16(p[i]);
       }
     }
     if (whole) {
@@ -318,8 +339,8 @@ __global__ __launch_bounds__(NT) void adamw_kernel(Table t, Moments st, Hyper h,
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         if (i >= n) continue;
-        while (seg + 1 < t.count && t.s[seg + 1].start <= first + i) ++seg;
-        ((T*)t.s[seg].p)[first + i - t.s[seg].start] = q[i];
+        while (seg + 1 < t.count && segs[seg + 1].start <= first + i) ++seg;
+        ((T*)segs[seg].p)[first + i - segs[seg].start] = q[i];
         if (EIGHT) {
           ((unsigned char*)st.m)[first + i] = (unsigned char)(cm[i / 4] >> (i % 4 * 8));
           ((unsigned char*)st.v)[first + i] = (unsigned char)(cv[i / 4] >> (i % 4 * 8));
@@ -341,39 +362,50 @@ __global__ __launch_bounds__(NT) void adamw_kernel(Table t, Moments st, Hyper h,
   }
 }
 
-// Both moments' values, 8 a thread.
+// The values of 8 codes.
 template <typename O, bool FIRST>
 __device__ __forceinline__ void decode8(const unsigned char* __restrict__ c,
                                         const unsigned char* __restrict__ e, int64_t first, int64_t P,
                                         bool whole, O* __restrict__ out) {
   const int ex = e[first / QB];
-  alignas(8) unsigned char in[8] = {};
-  alignas(16) O o[8];
   const int n = (int)min((int64_t)8, P - first);
+  alignas(8) unsigned int in[2] = {0, 0};
+  alignas(16) O o[8];
   if (whole && n == 8)
     *(uint2*)in = *(const uint2*)(c + first);
   else
-    for (int i = 0; i < n; ++i) in[i] = c[first + i];
+    for (int i = 0; i < n; ++i) in[i / 4] |= (unsigned int)c[first + i] << (i % 4 * 8);
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    o[i] = from_float<O>(Code<FIRST>::is_nan(in[i]) ? __uint_as_float(0x7FC00000u)
-                                                    : Code<FIRST>::decode(in[i], ex));
+    o[i] = from_float<O>(Code<FIRST>::decode(in[i / 4] >> (i % 4 * 8) & 255u, ex));
+  if (Code<FIRST>::odd_codes(in[0]) || Code<FIRST>::odd_codes(in[1])) {
+    MM_SELDOM();
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (Code<FIRST>::is_nan(in[i / 4] >> (i % 4 * 8) & 255u))
+        o[i] = from_float<O>(__uint_as_float(0x7FC00000u));
+  }
   if (n == 8) {
     constexpr int V = 16 / sizeof(O);
 #pragma unroll
     for (int i = 0; i < 8; i += V) *(Vec<O, V>*)(out + first + i) = *(const Vec<O, V>*)(o + i);
   } else {
-    for (int i = 0; i < n; ++i) out[first + i] = o[i];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) out[first + i] = o[i];
   }
 }
 
+// Both moments, 8 values of one a thread: blockIdx.y tells which.
 template <typename O>
 __global__ __launch_bounds__(NT) void adamw_decode_kernel(Moments st, int64_t P, O* __restrict__ m,
                                                           O* __restrict__ v) {
   const int64_t first = ((int64_t)blockIdx.x * NT + threadIdx.x) * 8;
   if (first >= P) return;
-  decode8<O, true>((const unsigned char*)st.m, st.me, first, P, st.whole, m);
-  decode8<O, false>((const unsigned char*)st.v, st.ve, first, P, st.whole, v);
+  if (blockIdx.y == 0)
+    decode8<O, true>((const unsigned char*)st.m, st.me, first, P, st.whole, m);
+  else
+    decode8<O, false>((const unsigned char*)st.v, st.ve, first, P, st.whole, v);
 }
 
 void check_state(const std::vector<Tensor>& s, int64_t P, const at::Device& d) {
@@ -507,8 +539,8 @@ std::tuple<Tensor, Tensor> adamw_decode(const std::vector<Tensor>& exp_avg,
              (unsigned char*)exp_avg_sq[1].data_ptr(), false};
   mo.whole = ((uintptr_t)mo.m | (uintptr_t)mo.v) % 8 == 0;
   MM_DISPATCH_TYPE(m, {
-    adamw_decode_kernel<T><<<(unsigned)blocks, NT, 0, stream_of(m)>>>(mo, P, (T*)m.data_ptr(),
-                                                                      (T*)v.data_ptr());
+    adamw_decode_kernel<T><<<dim3((unsigned)blocks, 2), NT, 0, stream_of(m)>>>(
+        mo, P, (T*)m.data_ptr(), (T*)v.data_ptr());
   });
   check_launch("adamw_dequantize");
   return {m, v};
