@@ -33,23 +33,53 @@ struct Epilogue {
   void* z;          // what the activation is taken of, or null
   void* out;
   int act;
+  bool whole;  // 8 columns of a row lie on 16 bytes, in all of these
 };
 
-__device__ __forceinline__ float activate(float z, int act) {
-  switch (act) {
-    case ACT_RELU: return act_fwd<ACT_RELU>(z);
-    case ACT_SILU: return act_fwd<ACT_SILU>(z);
-    case ACT_GELU: return act_fwd<ACT_GELU>(z);
-    default: return z;
-  }
-}
-
-template <typename T>
+template <typename T, int ACT>
 __device__ __forceinline__ void finish(const Epilogue& e, int64_t at, int64_t col, float v) {
   float z = v + load_param(e.bias, col, e.bias_float, 0.f);
   if (e.res) z += to_float(((const T*)e.res)[at]);
   if (e.z) ((T*)e.z)[at] = from_float<T>(z);
-  ((T*)e.out)[at] = from_float<T>(activate(z, e.act));
+  ((T*)e.out)[at] = from_float<T>(act_fwd<ACT>(z));
+}
+
+template <typename T>
+struct Eight {  // 8 values that lie on 16 bytes
+  static constexpr int V = 16 / sizeof(T);
+  Vec<T, V> v[8 / V];
+  __device__ __forceinline__ T& operator[](int i) { return v[i / V].e[i % V]; }
+  __device__ __forceinline__ void load(const void* p, int64_t at) {
+#pragma unroll
+    for (int i = 0; i < 8 / V; ++i) v[i] = ((const Vec<T, V>*)((const T*)p + at))[i];
+  }
+  __device__ __forceinline__ void store(void* p, int64_t at) const {
+#pragma unroll
+    for (int i = 0; i < 8 / V; ++i) ((Vec<T, V>*)((T*)p + at))[i] = v[i];
+  }
+};
+
+// 8 columns of a row, which lie on 16 bytes
+template <typename T, int ACT>
+__device__ __forceinline__ void finish8(const Epilogue& e, int64_t at, const float (&bias)[8],
+                                        const float* v) {
+  float z[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) z[i] = v[i] + bias[i];
+  Eight<T> o;
+  if (e.res) {
+    o.load(e.res, at);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) z[i] += to_float(o[i]);
+  }
+  if (e.z) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = from_float<T>(z[i]);
+    o.store(e.z, at);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o[i] = from_float<T>(act_fwd<ACT>(z[i]));
+  o.store(e.out, at);
 }
 
 template <typename T>
@@ -125,7 +155,7 @@ struct Stage {
 
 // Four waves side by side two by two, each with (BM/2) x (BN/2) of the tile in 16x16 blocks. A
 // lane holds 4 rows of one column of each block.
-template <typename T, bool AX, bool BX, int BM, int BN>
+template <typename T, bool AX, bool BX, int ACT, int BM, int BN>
 __global__ __launch_bounds__(NT) void gemm_kernel(Operand a, Operand b, int64_t M, int64_t N,
                                                   int64_t Kd, int64_t k_part, int64_t col_tiles,
                                                   Epilogue e, float* __restrict__ ws) {
@@ -198,19 +228,334 @@ __global__ __launch_bounds__(NT) void gemm_kernel(Operand a, Operand b, int64_t 
         if (ws)
           ws[(blockIdx.y * M + r) * N + c] = acc[i][j][q];
         else
-          finish<T>(e, r * N + c, c, acc[i][j][q]);
+          finish<T, ACT>(e, r * N + c, c, acc[i][j][q]);
       }
 }
 
-// joins the parts of a split sum, in their order
+// ------------------------------------------------------------ large products
+//
+// A block of WM x WN waves takes a tile of BM x BN, over 128 bytes of k at a time (64 values in bf16,
+// on which the text below counts, 32 in fp32). The operands' tiles go
+// from memory to LDS without registers between, into two buffers in turn. A wave multiplies a step
+// in four quarters and reads the fragments of the next quarter beside the products of this one:
+//
+//   1  upper rows, k 0..31      read A's upper rows and B, k 32..63
+//      wait, barrier X: A's upper rows and B are read; the lower rows have to be there
+//   2  upper rows, k 32..63     load A's upper rows and B of two steps ahead over them
+//                               read the lower rows, k 0..31
+//   3  lower rows, k 0..31      read the lower rows, k 32..63
+//      wait, barrier Y: the lower rows are read; the next step's upper rows and B have to be there
+//   4  lower rows, k 32..63     load the lower rows of two steps ahead; read the next step's first
+//
+// Upper and lower rows are halves of each wave's own, and lie in buffers of their own. So every load
+// has six quarters until it is waited for, with two buffers, and lines of 128 bytes are loaded whole.
+// (One barrier a step, and loads a step ahead, reached 1030 to 1130 TFLOP/s at 8192x4096x12288, tiles
+// of 32 of k four steps ahead 990 with half lines and 1180 with whole ones.)
+//
+// The loads are written in assembly, and waited for by count: the compiler would wait for all of
+// them before each transposing read. They have no result in registers, and a wait that it counts
+// without them only waits for more.
+//
+// LDS holds what a wave loaded in lane order, so the order that spares bank conflicts is made where
+// lanes choose what they load:
+// (A fragment is 16 bytes of each of 16 rows' k for 4 groups of 16 lanes: one bf16 product over 32 of
+// k, or four fp32 ones over 4 each, of which group q takes k = 4q + j in the j-th.)
+//   k along the rows:  [row][64], 16-byte chunk c of a row stands at c ^ (row / 2 & 7): 16 rows of
+//                      one chunk, which are read at once, lie in the 16 places of 256 bytes
+//   k across the rows: [k][rows], 16 columns of row k stand at their place ^ g(k); the fragments
+//                      come through the transposing read, 4 rows of k for 16 lanes, or value by
+//                      value in fp32
+// Rows behind the operand's end repeat its last ones (their results are not stored); the k behind
+// its end are zeros, put there through registers in a step of their own.
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) s4 lds_s4;
+
+constexpr int ROW_BYTES = 128;
+
+// ROWS rows of an operand: HR of each STRIDE, from the first on
+template <typename T, bool ACROSS, int ROWS, int THREADS, int HR, int STRIDE>
+struct Direct {
+  static constexpr int E = 16 / sizeof(T), FK = ROW_BYTES / sizeof(T);  // values of a chunk, of a row
+  static constexpr int LOADS = ROWS * (FK / E) / THREADS;
+  static constexpr int SIZE = ROWS * FK;
+  static constexpr int CH = ROWS / E;        // chunks of a row of k
+  static constexpr int PAIRS = ROWS / 16;    // 16 columns of it
+  static constexpr int LOW = PAIRS < 4 ? PAIRS - 1 : 3, HIGH = PAIRS < 4 ? 0 : PAIRS / 4 - 1;
+  const T* base;        // the tile, the same for all lanes
+  unsigned at[LOADS];   // a lane's places from there, in bytes
+  int64_t step;
+
+  __device__ __forceinline__ static int g_of(int k) {
+    return sizeof(T) == 4 ? (k >> 2) & LOW : (k & LOW) | ((k >> 3) & HIGH) << 2;
+  }
+  __device__ __forceinline__ static void slot(int i, int& r, int& k) {
+    const int s = i * THREADS + threadIdx.x;
+    if (ACROSS) {
+      k = s / CH;
+      r = ((s % CH) ^ g_of(k) * (16 / E)) * E;
+    } else {
+      r = s / 8;
+      k = ((s % 8) ^ (r >> 1 & 7)) * E;
+    }
+  }
+  __device__ __forceinline__ void init(const Operand& o, int64_t r0, int64_t k0, int64_t R) {
+    step = ACROSS ? FK * o.ld : FK;
+    r0 = min(r0, R - (ACROSS ? E : 1));  // rows that start behind the end
+    base = (const T*)o.p + (ACROSS ? k0 * o.ld + r0 : r0 * o.ld + k0);
+    const int last = (int)min(R - r0, (int64_t)(ROWS / HR * STRIDE)) - (ACROSS ? E : 1);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      int r, k;
+      slot(i, r, k);
+      r = min(r / HR * STRIDE + r % HR, last);
+      at[i] = (unsigned)(ACROSS ? k * o.ld + r : r * o.ld + k) * sizeof(T);
+    }
+  }
+  // `wave` the same for all lanes
+  __device__ __forceinline__ void load(T* lds, int wave) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const unsigned to = (unsigned)(uintptr_t)(lds_void*)(lds + (i * THREADS + wave * 64) * E);
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                   :
+                   : "s"(to), "v"(at[i]), "s"(base)
+                   : "memory");
+    }
+    base += step;
+  }
+  // the `left` values of k behind `steps` whole tiles
+  __device__ __forceinline__ void load_tail(T* lds, int64_t steps, int left) const {
+    const T* p = base + steps * step;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      int r, k;
+      slot(i, r, k);
+      const T* from = p + at[i] / sizeof(T);
+      Vec<T, E> v = {};
+      if ((ACROSS ? k + 1 : k + E) <= left) {
+        v = *(const Vec<T, E>*)from;
+      } else if (!ACROSS) {
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          if (k + j < left) v.e[j] = from[j];
+      }
+      *(Vec<T, E>*)(lds + (i * THREADS + threadIdx.x) * E) = v;
+    }
+  }
+  // 16 rows from `row`, half ks of the step's k: lane l has row l % 16, chunk l / 16 of the half
+  __device__ __forceinline__ static u4 fragment(const T* lds, int row, int ks) {
+    const int lane = threadIdx.x & 63, l = lane & 15, q = lane >> 4;
+    if constexpr (!ACROSS) {
+      return *(const u4*)(lds + (row + l) * FK + (((ks * 4 + q) ^ (l >> 1 & 7)) * E));
+    } else if constexpr (sizeof(T) == 2) {
+      const int g = ((l >> 2) & LOW) | (q & HIGH) << 2;
+      const T* p = lds + (ks * 32 + q * 8 + (l >> 2)) * ROWS + ((row >> 4) ^ g) * 16 + (l & 3) * 4;
+      union {
+        s4 h[2];
+        u4 v;
+      } f;
+      f.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)p);
+      f.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + 4 * ROWS));
+      return f.v;
+    } else {
+      const T* p = lds + (ks * 16 + q * 4) * ROWS + ((row >> 4) ^ (q & LOW)) * 16 + l;
+      u4 f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[j] = __float_as_uint(p[j * ROWS]);
+      return f;
+    }
+  }
+};
+
 template <typename T>
+__device__ __forceinline__ f4 product(u4 a, u4 b, f4 c) {
+  if constexpr (sizeof(T) == 2) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
+    return c;
+  }
+}
+
+// which tile a block takes: blocks of one XCD (every eighth) take neighbours, 8 tiles down before
+// the next column, so that what they share stays in that XCD's L2
+__device__ __forceinline__ void tile_of(int64_t b, int64_t rows, int64_t cols, int64_t& r, int64_t& c) {
+  const int64_t total = rows * cols, each = total / 8, rest = total % 8, x = b % 8;
+  const int64_t t = x * each + min(x, rest) + b / 8;
+  const int64_t band = 8 * cols, top = t / band * 8, height = min((int64_t)8, rows - top);
+  r = top + t % band % height;
+  c = t % band / height;
+}
+
+template <typename T, bool AX, bool BX, int ACT, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, 2) void gemm_large_kernel(
+    Operand a, Operand b, int64_t M, int64_t N, int64_t Kd, int64_t a_end, int64_t b_end, int64_t k_part,
+    int64_t row_tiles, int64_t col_tiles, Epilogue e, float* __restrict__ ws) {
+  constexpr int THREADS = 64 * WM * WN, FM = BM / WM / 16, FN = BN / WN / 16, H = FM / 2;
+  using A = Direct<T, AX, BM / 2, THREADS, H * 16, FM * 16>;  // the upper rows, or the lower ones
+  using B = Direct<T, BX, BN, THREADS, BN, BN>;
+  constexpr int FK = A::FK;
+  __shared__ __attribute__((aligned(1024))) T lds[2 * (2 * A::SIZE + B::SIZE)];
+  // per buffer: upper rows, lower rows, B
+  const auto up = [&](int at) { return lds + at * (2 * A::SIZE + B::SIZE); };
+  const auto low = [&](int at) { return up(at) + A::SIZE; };
+  const auto bs = [&](int at) { return up(at) + 2 * A::SIZE; };
+  int64_t tr, tc;
+  tile_of(blockIdx.x, row_tiles, col_tiles, tr, tc);
+  const int64_t m0 = tr * BM, n0 = tc * BN;
+  const int64_t kb = blockIdx.y * k_part, ke = min(Kd, kb + k_part);
+  const int tiles = (int)((max(ke, kb) - kb) / FK), left = (int)((max(ke, kb) - kb) % FK);
+  const int steps = tiles + (left > 0);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+  A du, dl;
+  B db;
+  du.init(a, m0, kb, a_end);
+  dl.init(a, m0 + H * 16, kb, a_end);
+  db.init(b, n0, kb, b_end);
+  // what is left over of k comes first
+  if (left > 0) {
+    du.load_tail(up(0), tiles, left);
+    dl.load_tail(low(0), tiles, left);
+    db.load_tail(bs(0), tiles, left);
+  }
+  for (int s = left > 0; s < min(steps, 2); ++s) {
+    du.load(up(s), wave);
+    db.load(bs(s), wave);
+    dl.load(low(s), wave);
+  }
+  f4 acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) acc[i][j] = {0.f, 0.f, 0.f, 0.f};
+  u4 a0[H], a1[H], b0[FN], b1[FN];
+  const auto read_a = [&](u4 (&f)[H], const T* tile, int ks) {
+#pragma unroll
+    for (int i = 0; i < H; ++i) f[i] = A::fragment(tile, wave / WN * (H * 16) + i * 16, ks);
+  };
+  const auto read_b = [&](u4 (&f)[FN], const T* tile, int ks) {
+#pragma unroll
+    for (int j = 0; j < FN; ++j) f[j] = B::fragment(tile, wn + j * 16, ks);
+  };
+  const auto multiply = [&](const u4 (&fa)[H], const u4 (&fb)[FN], int half) {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int i = 0; i < H; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+        acc[half * H + i][j] = product<T>(fb[j], fa[i], acc[half * H + i][j]);
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // A step's loads but the oldest of them may still be on their way at a barrier; at the sum's end,
+  // where nothing new is loaded, all are waited for.
+  constexpr int AHEAD = 2 * A::LOADS + B::LOADS;
+  const auto barrier = [&](bool all) {
+    if (all)
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(AHEAD) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  barrier(true);
+  read_b(b0, bs(0), 0);
+  read_a(a0, up(0), 0);
+#pragma unroll 1
+  for (int s = 0; s < steps; ++s) {
+    const int at = s & 1;
+    const bool more = s + 2 < steps;
+    read_b(b1, bs(at), 1);
+    read_a(a1, up(at), 1);
+    multiply(a0, b0, 0);
+    barrier(!more);
+    read_a(a0, low(at), 0);
+    if (more) {
+      du.load(up(at), wave);
+      db.load(bs(at), wave);
+    }
+    multiply(a1, b1, 0);
+    read_a(a1, low(at), 1);
+    multiply(a0, b0, 1);
+    barrier(!more);
+    // the last step reads on, into a tile that nobody needs
+    read_b(b0, bs(at ^ 1), 0);
+    read_a(a0, up(at ^ 1), 0);
+    if (more) dl.load(low(at), wave);
+    multiply(a1, b1, 1);
+  }
+  // A lane has 4 neighbouring columns of a row in each block.
+  if (ws) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      const int64_t r = m0 + wm + i * 16 + (lane & 15);
+      float* row = ws + (blockIdx.y * M + r) * N;
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        const int64_t c = n0 + wn + j * 16 + (lane >> 4) * 4;
+        if (r >= M) continue;
+        if (N % 4 == 0 && c < N) {
+          *(f4*)(row + c) = acc[i][j];
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (c + q < N) row[c + q] = acc[i][j][q];
+        }
+      }
+    }
+    return;
+  }
+  // Through LDS, a wave 32 of its rows at a time, so that each lane finishes 8 columns of one row
+  // and rows leave in whole lines. 4 floats more a row keep 8 rows' writes in different banks.
+  constexpr int COLS = BN / WN, PITCH = COLS + 4, LANES = COLS / 8, DOWN = 64 / LANES;
+  static_assert(64 % COLS == 0 && FM % 2 == 0 && WM * WN * 32 * PITCH * 4 <= sizeof(lds), "");
+  __syncthreads();
+  float* mine = (float*)lds + wave * 32 * PITCH;
+  const bool inside = e.whole && m0 + BM <= M && n0 + BN <= N;
+  const int64_t c = n0 + wn + lane % LANES * 8;
+  float bias[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) bias[q] = c + q < N ? load_param(e.bias, c + q, e.bias_float, 0.f) : 0.f;
+#pragma unroll
+  for (int i = 0; i < FM; i += 2) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+        *(f4*)(mine + (h * 16 + (lane & 15)) * PITCH + j * 16 + (lane >> 4) * 4) = acc[i + h][j];
+    __builtin_amdgcn_wave_barrier();
+    const float* row = mine + lane / LANES * PITCH + lane % LANES * 8;
+    const int64_t r = m0 + wm + i * 16 + lane / LANES;
+    if (inside) {
+#pragma unroll
+      for (int k = 0; k < 32; k += DOWN) finish8<T, ACT>(e, (r + k) * N + c, bias, row + k * PITCH);
+    } else {  // a row at a time, a value a lane
+      const int64_t one = n0 + wn + lane % COLS;
+#pragma unroll 4
+      for (int k = lane / COLS; k < 32; k += 64 / COLS) {
+        const int64_t down = m0 + wm + i * 16 + k;
+        if (down < M && one < N) finish<T, ACT>(e, down * N + one, one, mine[k * PITCH + lane % COLS]);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// joins the parts of a split sum, in their order
+template <typename T, int ACT>
 __global__ __launch_bounds__(NT) void join_kernel(const float* __restrict__ ws, int parts,
                                                   int64_t total, int64_t N, Epilogue e) {
   const int64_t at = (int64_t)blockIdx.x * NT + threadIdx.x;
   if (at >= total) return;
   float v = 0.f;
   for (int s = 0; s < parts; ++s) v += ws[s * total + at];
-  finish<T>(e, at, at % N, v);
+  finish<T, ACT>(e, at, at % N, v);
 }
 
 // dz = dy * act'(z) and, for each chunk of rows, its sum over them. 64 columns a block, a wave a
@@ -266,19 +611,111 @@ __global__ __launch_bounds__(NT) void bias_grad_kernel(const float* __restrict__
 const void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 Operand operand(const Tensor& t) {
-  const int64_t size = t.element_size();
-  return {t.data_ptr(), t.stride(0), t.stride(0) * size % 16 == 0 && (uintptr_t)t.data_ptr() % 16 == 0};
+  const int64_t size = t.element_size(), ld = t.size(0) > 1 ? t.stride(0) : 0;
+  return {t.data_ptr(), ld, ld * size % 16 == 0 && (uintptr_t)t.data_ptr() % 16 == 0};
 }
 
-template <typename T, bool AX, bool BX, int B>
-void launch_gemm(const Operand& a, const Operand& b, int64_t M, int64_t N, int64_t Kd, int64_t parts,
-                 const Epilogue& e, float* ws, hipStream_t st) {
-  const int64_t rows = ceil_div(M, B), cols = ceil_div(N, B);
+bool rows_of_8(int64_t N, std::initializer_list<const void*> ptrs) {
+  if (N % 8) return false;
+  for (const void* p : ptrs)
+    if ((uintptr_t)p % 16) return false;
+  return true;
+}
+
+// Up to two matrices, copied so that each row starts on 16 bytes, with zeros behind the values and
+// in the rows behind `full`.
+struct Pad {
+  Operand from;
+  int64_t full, cols;  // rows and columns that there are
+  int64_t rows, ld;    // and with those behind them
+  void* to;
+};
+
+template <typename T>
+__global__ __launch_bounds__(NT) void pad_kernel(Pad a, Pad b) {
+  const bool second = (int64_t)blockIdx.x >= a.rows;
+  const Pad& p = second ? b : a;
+  const int64_t row = second ? blockIdx.x - a.rows : blockIdx.x;
+  const T* from = (const T*)p.from.p + row * p.from.ld;
+  T* to = (T*)p.to + row * p.ld;
+  for (int64_t c = threadIdx.x; c < p.ld; c += NT) to[c] = row < p.full && c < p.cols ? from[c] : T{};
+}
+
+struct Choice {
+  int tile;
+  int64_t parts;
+};
+
+struct TileShape {
+  int bm, bn, per_cu;
+  // microseconds that a step of 128 bytes of k takes on a CU with 1, 2, 3 such blocks
+  double bf16_us[4], fp32_us[4];
+};
+constexpr TileShape TILES[] = {
+    {256, 256, 1, {1.80}, {7.0}},
+    {256, 128, 1, {0.97}, {3.6}},
+    {128, 128, 2, {0.67, 1.03}, {1.85, 3.6}},
+    {64, 64, 4, {0.45, 0.50, 0.70, 0.90}, {0.60, 0.95, 1.40, 1.85}},
+};
+
+// Which tile, and into how many parts the sum is split: the least of an estimate. A tile's steps are
+// measured at 4096 and 8192 rows and columns with all CUs busy, and with one block a CU, where what
+// it waits for shows. A split costs its parts' writing and reading at 5 TB/s and a launch; and no
+// choice is faster than memory, which some hundred blocks are needed to keep busy. The choice is
+// within 15% of the best of all tiles and splits over 22 products that were measured, from 33x200x40
+// on. bf16, M x K x N: 2048x12288x4096 takes 278 us in tiles of 256x256 and 205 in two parts, 184 in
+// 256x128, 198 in 128x128; 1024x1024x1024 14 in 128x128, 9 in 64x64; 64x3136x2048 19 in 64x64 whole,
+// 8.5 in 8 parts; 1x4096x12288 39 whole, 19 in 2 parts, 22 in 8.
+Choice choose(int64_t M, int64_t N, int64_t Kd, int64_t elem) {
+  Choice best{0, 1};
+  double least = 1e30;
+  const int64_t steps = ceil_div(Kd * elem, ROW_BYTES);
+  const double bytes = (double)(M * Kd + N * Kd + M * N) * elem;
+  for (int t = 0; t < 4; ++t) {
+    const TileShape& s = TILES[t];
+    const int64_t tiles = ceil_div(M, s.bm) * ceil_div(N, s.bn);
+    for (int64_t parts = 1; parts <= 64 && (parts == 1 || (steps >= 2 * parts && tiles * parts <= 1536));
+         parts *= 2) {
+      const int64_t a_cu = ceil_div(tiles * parts, 256), full = a_cu / s.per_cu, rest = a_cu % s.per_cu;
+      const double* us = elem == 2 ? s.bf16_us : s.fp32_us;
+      const double part = (double)ceil_div(steps, parts);
+      double cost = full * (part * us[s.per_cu - 1] + 2) + (rest ? part * us[rest - 1] + 2 : 0);
+      cost = std::max(cost, bytes / 5e6 * std::max(1.0, 256.0 / (tiles * parts)));
+      if (parts > 1) cost += 6 + (double)M * N * 8 * parts / 5e6;
+      if (cost < least) {
+        least = cost;
+        best = {t, parts};
+      }
+    }
+  }
+  return best;
+}
+
+template <typename T, bool AX, bool BX, int ACT, int BM, int BN, int WM, int WN>
+void launch_large(const Operand& a, const Operand& b, int64_t M, int64_t N, int64_t Kd, int64_t Ma,
+                  int64_t Nb, int64_t parts, const Epilogue& e, float* ws, hipStream_t st) {
+  const int64_t rows = ceil_div(M, BM), cols = ceil_div(N, BN), values = ROW_BYTES / sizeof(T);
+  TORCH_CHECK(rows * cols < (1LL << 31), "linear_act: too many tiles");
+  const int64_t part = ceil_div(ceil_div(Kd, parts), values) * values;
+  gemm_large_kernel<T, AX, BX, ACT, BM, BN, WM, WN>
+      <<<dim3((unsigned)(rows * cols), (unsigned)parts), 64 * WM * WN, 0, st>>>(a, b, M, N, Kd, Ma, Nb, part,
+                                                                              rows, cols, e, ws);
+}
+
+template <typename T, bool AX, bool BX, int ACT>
+void launch_small(const Operand& a, const Operand& b, int64_t M, int64_t N, int64_t Kd, int64_t parts,
+                  const Epilogue& e, float* ws, hipStream_t st) {
+  const int64_t rows = ceil_div(M, 64), cols = ceil_div(N, 64);
   TORCH_CHECK(rows * cols < (1LL << 31), "linear_act: too many tiles");
   const int64_t part = ceil_div(ceil_div(Kd, parts), Tile<T>::BK) * Tile<T>::BK;
-  gemm_kernel<T, AX, BX, B, B><<<dim3((unsigned)(rows * cols), (unsigned)parts), NT, 0, st>>>(
+  gemm_kernel<T, AX, BX, ACT, 64, 64><<<dim3((unsigned)(rows * cols), (unsigned)parts), NT, 0, st>>>(
       a, b, M, N, Kd, part, cols, e, ws);
 }
+
+// A product of rows off the 16 bytes is worth a copy of them from this many multiplications on:
+// 509x561x250 in bf16 takes 13 us as it lies and 21 with the copy, 2000x561x250 20 and 22,
+// 1000x1001x999 43 and 27, 4001x4003x4099 2435 and 198.
+constexpr double PAD_FROM = 8e8;
 
 // out [M, N] = A B^T over Kd, A and B with k along (or across) their rows in memory
 template <bool AX, bool BX>
@@ -286,22 +723,64 @@ void gemm(const Tensor& a, const Tensor& b, int64_t M, int64_t N, int64_t Kd, co
           const Tensor& like) {
   if (M == 0 || N == 0) return;
   const hipStream_t st = stream_of(like);
-  const bool large = ceil_div(M, 128) * ceil_div(N, 128) >= 256;
-  const int64_t B = large ? 128 : 64;
-  const int64_t tiles = ceil_div(M, B) * ceil_div(N, B);
-  // few tiles: the sum is split over k, 128 values a part at least
-  const int64_t parts = std::max<int64_t>(1, std::min(ceil_div(512, tiles), Kd / 128));
-  Tensor ws;
-  if (parts > 1) ws = at::empty({parts * M * N}, like.options().dtype(at::kFloat));
-  float* wp = parts > 1 ? ws.data_ptr<float>() : nullptr;
-  const Operand oa = operand(a), ob = operand(b);
-  MM_DISPATCH_TYPE(like, {
-    if (large) launch_gemm<T, AX, BX, 128>(oa, ob, M, N, Kd, parts, e, wp, st);
-    else launch_gemm<T, AX, BX, 64>(oa, ob, M, N, Kd, parts, e, wp, st);
-    if (parts > 1) {
-      TORCH_CHECK(ceil_div(M * N, NT) < (1LL << 31), "linear_act: too many values");
-      join_kernel<T><<<(unsigned)ceil_div(M * N, NT), NT, 0, st>>>(wp, (int)parts, M * N, N, e);
+  Operand oa = operand(a), ob = operand(b);
+  const int64_t elem = like.element_size(), E = 16 / elem;
+  // offsets within a tile are 32 bits
+  bool large = Kd > 0 && std::max(oa.ld, ob.ld) * 256 * elem < (1LL << 32);
+  const bool fits_a = oa.whole && (!AX || M % E == 0), fits_b = ob.whole && (!BX || N % E == 0);
+  int64_t Ma = M, Nb = N;  // rows that may be read
+  Tensor padded;
+  if (large && !(fits_a && fits_b)) {
+    large = (double)M * N * Kd >= PAD_FROM;
+    if (large) {
+      // k is filled up to whole steps with zeros, the rows that a product goes over to whole vectors
+      const int64_t step = ROW_BYTES / elem;
+      const auto pad = [&](const Tensor& t, const Operand& o, bool fits, bool across) {
+        if (fits) return Pad{o, 0, 0, 0, 0, nullptr};
+        return Pad{o, t.size(0), t.size(1), across ? ceil_div(t.size(0), step) * step : t.size(0),
+                   across ? ceil_div(t.size(1), E) * E : ceil_div(t.size(1), step) * step, nullptr};
+      };
+      Pad pa = pad(a, oa, fits_a, AX), pb = pad(b, ob, fits_b, BX);
+      padded = at::empty({pa.rows * pa.ld + pb.rows * pb.ld}, like.options());
+      TORCH_CHECK(pa.rows + pb.rows < (1LL << 31), "linear_act: too many rows");
+      pa.to = padded.data_ptr();
+      pb.to = (char*)pa.to + pa.rows * pa.ld * elem;
+      MM_DISPATCH_TYPE(like, (pad_kernel<T><<<(unsigned)(pa.rows + pb.rows), NT, 0, st>>>(pa, pb)));
+      if (!fits_a) oa = {pa.to, pa.ld, true}, Ma = AX ? pa.ld : M;
+      if (!fits_b) ob = {pb.to, pb.ld, true}, Nb = BX ? pb.ld : N;
+      if (!fits_a && !fits_b) Kd = ceil_div(Kd, step) * step;
     }
+  }
+  Choice c{0, 1};
+  if (large) {
+    c = choose(M, N, Kd, elem);
+  } else {
+    // few tiles: the sum is split over k, 128 values a part at least
+    c.parts = std::max<int64_t>(1, std::min(ceil_div(512, ceil_div(M, 64) * ceil_div(N, 64)), Kd / 128));
+  }
+  Tensor ws;
+  if (c.parts > 1) ws = at::empty({c.parts * M * N}, like.options().dtype(at::kFloat));
+  float* wp = c.parts > 1 ? ws.data_ptr<float>() : nullptr;
+  MM_DISPATCH_TYPE(like, {
+    MM_DISPATCH_ACT((AX || BX) ? 0 : e.act, {
+      if constexpr (ACT == ACT_NONE || !(AX || BX)) {  // only the forward product has an epilogue
+        if (!large)
+          launch_small<T, AX, BX, ACT>(oa, ob, M, N, Kd, c.parts, e, wp, st);
+        else if (c.tile == 0)
+          launch_large<T, AX, BX, ACT, 256, 256, 2, 4>(oa, ob, M, N, Kd, Ma, Nb, c.parts, e, wp, st);
+        else if (c.tile == 1)
+          launch_large<T, AX, BX, ACT, 256, 128, 4, 2>(oa, ob, M, N, Kd, Ma, Nb, c.parts, e, wp, st);
+        else if (c.tile == 2)
+          launch_large<T, AX, BX, ACT, 128, 128, 2, 2>(oa, ob, M, N, Kd, Ma, Nb, c.parts, e, wp, st);
+        else
+          launch_large<T, AX, BX, ACT, 64, 64, 2, 2>(oa, ob, M, N, Kd, Ma, Nb, c.parts, e, wp, st);
+        if (c.parts > 1) {
+          TORCH_CHECK(ceil_div(M * N, NT) < (1LL << 31), "linear_act: too many values");
+          join_kernel<T, ACT>
+              <<<(unsigned)ceil_div(M * N, NT), NT, 0, st>>>(wp, (int)c.parts, M * N, N, e);
+        }
+      }
+    });
   });
   check_launch("linear_act");
 }
@@ -336,7 +815,7 @@ Forward forward_of(const Tensor& x, const Tensor& weight, const Tensor& bias, co
   const bool keep_z = differentiable && (act == ACT_SILU || act == ACT_GELU);
   if (keep_z) f.keep = at::empty(sizes, x.options());
   Epilogue e{ptr(b), b.defined() && b.scalar_type() == at::kFloat, ptr(res), (void*)ptr(f.keep),
-             f.y.data_ptr(), (int)act};
+             f.y.data_ptr(), (int)act, rows_of_8(N, {ptr(res), ptr(f.keep), ptr(f.y)})};
   gemm<false, false>(f.x, f.w, M, N, Kd, e, x);
   if (differentiable && act == ACT_RELU) f.keep = f.y;
   return f;
@@ -399,12 +878,12 @@ class LinearAct : public torch::autograd::Function<LinearAct> {
     Tensor dx, dw;
     if (needs & 1) {
       dx = at::empty(sizes, dy.options());
-      Epilogue e{nullptr, false, nullptr, nullptr, dx.data_ptr(), ACT_NONE};
+      Epilogue e{nullptr, false, nullptr, nullptr, dx.data_ptr(), ACT_NONE, rows_of_8(Kd, {ptr(dx)})};
       gemm<false, true>(dzm, saved[1], M, Kd, N, e, dy);
     }
     if (needs & 2) {
       dw = at::empty({N, Kd}, dy.options());
-      Epilogue e{nullptr, false, nullptr, nullptr, dw.data_ptr(), ACT_NONE};
+      Epilogue e{nullptr, false, nullptr, nullptr, dw.data_ptr(), ACT_NONE, rows_of_8(Kd, {ptr(dw)})};
       gemm<true, true>(dzm, saved[0], N, Kd, M, e, dy);
     }
     return {dx, dw, db, needs & 8 ? dz : Tensor(), Tensor()};
