@@ -342,6 +342,242 @@ __global__ __launch_bounds__(1024) void gn_bwd_params_kernel(const float2* __res
   }
 }
 
+// --------------------------------------------- a tile of groups in registers
+//
+// Where all pixels of some whole groups fit into a block's registers, the block reads them once:
+// it has their mean, their variance and the result (going back: the sums and dx) without looking at
+// memory again. Blocks that share lines of memory, the tiles of one sample, run on one XCD.
+struct Tile {
+  int64_t R;
+  int C, G, Cg;
+  int groups;     // of the tile
+  int lanes;      // log2 of the lanes along the channels, the last of which may be idle
+  int tiles;      // of a sample
+  int64_t blocks;
+};
+
+constexpr int MAX_WAVES = 16;
+constexpr int MAX_CHANNELS = 512;
+
+struct Spot {
+  int64_t n;
+  int tile, c0, col, row, step;  // first channel; the lane's first in the tile; first row, rows a pass
+  bool active;
+};
+
+template <int V>
+__device__ __forceinline__ Spot spot_of(const Tile& t) {
+  Spot p;
+  const int64_t each = t.blocks / 8, rest = t.blocks % 8, x = blockIdx.x % 8;
+  const int64_t b = x * each + min(x, rest) + blockIdx.x / 8;
+  p.n = b / t.tiles;
+  p.tile = (int)(b % t.tiles);
+  p.c0 = p.tile * t.groups * t.Cg;
+  p.col = (threadIdx.x & ((1 << t.lanes) - 1)) * V;
+  p.row = threadIdx.x >> t.lanes;
+  p.step = blockDim.x >> t.lanes;
+  p.active = p.col < t.groups * t.Cg;
+  return p;
+}
+
+// sums of `part` [waves][pitch] over waves and the channels of each group, one wave a group
+__device__ __forceinline__ void over_groups(const float* part, const Tile& t, int pitch, float* to) {
+  const int waves = blockDim.x >> 6, lane = threadIdx.x & 63;
+  for (int g = threadIdx.x >> 6; g < t.groups; g += waves) {
+    float s = 0.f;
+    for (int c = lane % t.Cg, w = lane / t.Cg, stop = 64 / t.Cg * t.Cg; lane < stop && w < waves;
+         w += 64 / t.Cg)
+      s += part[w * pitch + g * t.Cg + c];
+    if (t.Cg > 64) {
+      s = 0.f;
+      for (int w = 0; w < waves; ++w)
+        for (int c = lane; c < t.Cg; c += 64) s += part[w * pitch + g * t.Cg + c];
+    }
+    s = wave_sum(s);
+    if (lane == 0) to[g] = s;
+  }
+}
+
+template <typename T, int V, int ACT, int KR>
+__global__ __launch_bounds__(1024) void gn_tile_kernel(
+    const T* __restrict__ x, const T* __restrict__ res, Tile t, float eps, const void* __restrict__ gamma,
+    const void* __restrict__ beta, bool wf, T* __restrict__ y, float* __restrict__ mean,
+    float* __restrict__ rstd) {
+  __shared__ float part[MAX_WAVES * 64 * V];
+  __shared__ float group[MAX_CHANNELS], spread[MAX_CHANNELS];
+  const Spot p = spot_of<V>(t);
+  const int pitch = V << t.lanes;
+  const float inv = 1.f / ((float)t.R * (float)t.Cg);
+  const int64_t first = (p.n * t.R + p.row) * t.C + p.c0 + p.col, stride = (int64_t)p.step * t.C;
+  int g[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) g[v] = p.active ? (p.col + v) / t.Cg : 0;
+  Packed<T, V> val[KR];
+  float acc[V] = {};
+#pragma unroll
+  for (int i = 0; i < KR; ++i)
+    if (p.active && p.row + i * p.step < t.R) val[i].load(x + first + i * stride);
+#pragma unroll
+  for (int i = 0; i < KR; ++i)
+    if (p.active && p.row + i * p.step < t.R) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[v] += val[i].get(v);
+    }
+  rows_to_waves<V>(acc, t.lanes, p.col / V, part);
+  __syncthreads();
+  over_groups(part, t, pitch, group);
+  __syncthreads();
+  float mu[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) mu[v] = group[g[v]] * inv, acc[v] = 0.f;
+#pragma unroll
+  for (int i = 0; i < KR; ++i)
+    if (p.active && p.row + i * p.step < t.R) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const float d = val[i].get(v) - mu[v];
+        acc[v] += d * d;
+      }
+    }
+  rows_to_waves<V>(acc, t.lanes, p.col / V, part);
+  __syncthreads();
+  over_groups(part, t, pitch, spread);
+  __syncthreads();
+  for (int i = threadIdx.x; i < t.groups; i += blockDim.x) {
+    const int64_t at = p.n * t.G + p.tile * t.groups + i;
+    mean[at] = group[i] * inv;
+    rstd[at] = 1.f / sqrtf(spread[i] * inv + eps);
+  }
+  if (!p.active) return;
+  float rs[V], ga[V], be[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    rs[v] = 1.f / sqrtf(spread[g[v]] * inv + eps);
+    ga[v] = load_param(gamma, p.c0 + p.col + v, wf, 1.f);
+    be[v] = load_param(beta, p.c0 + p.col + v, wf, 0.f);
+  }
+#pragma unroll
+  for (int i = 0; i < KR; ++i)
+    if (p.row + i * p.step < t.R) {
+      Packed<T, V> r = {}, o;
+      if (res) r.load(res + first + i * stride);
+      float z[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        z[v] = act_fwd<ACT>((val[i].get(v) - mu[v]) * rs[v] * ga[v] + be[v] + r.get(v));
+#pragma unroll
+      for (int v = 0; v < V / 2; ++v) o.set2(v, z[2 * v], z[2 * v + 1]);
+      o.store(y + first + i * stride);
+    }
+}
+
+template <typename T, int V, int ACT, int KR>
+__global__ __launch_bounds__(512) void gn_tile_bwd_kernel(
+    const T* __restrict__ x, const T* __restrict__ dy, const T* __restrict__ res, Tile t,
+    const float* __restrict__ mean, const float* __restrict__ rstd, const void* __restrict__ gamma,
+    const void* __restrict__ beta, bool wf, T* __restrict__ dx, T* __restrict__ dres,
+    float2* __restrict__ ws) {
+  __shared__ float part[2][8 * 64 * V];
+  __shared__ float group[2][MAX_CHANNELS];
+  const Spot p = spot_of<V>(t);
+  const int pitch = V << t.lanes, waves = blockDim.x >> 6;
+  const int64_t first = (p.n * t.R + p.row) * t.C + p.c0 + p.col, stride = (int64_t)p.step * t.C;
+  Packed<T, V> xv[KR], dv[KR];
+#pragma unroll
+  for (int i = 0; i < KR; ++i)
+    if (p.active && p.row + i * p.step < t.R) {
+      xv[i].load(x + first + i * stride);
+      dv[i].load(dy + first + i * stride);
+    }
+  int g[V];
+  float mu[V], rs[V], ga[V], be[V], sz[V] = {}, sx[V] = {};
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    g[v] = p.active ? (p.col + v) / t.Cg : 0;
+    const int64_t at = p.n * t.G + p.tile * t.groups + g[v];
+    const int c = p.active ? p.c0 + p.col + v : p.c0;
+    mu[v] = mean[at];
+    rs[v] = rstd[at];
+    ga[v] = load_param(gamma, c, wf, 1.f);
+    be[v] = load_param(beta, c, wf, 0.f);
+  }
+  // dz of a value, from what the registers hold
+  const auto through = [&](int i, int v, float r, float& xh) {
+    xh = (xv[i].get(v) - mu[v]) * rs[v];
+    return act_bwd<ACT>(dv[i].get(v), xh * ga[v] + be[v] + r);
+  };
+#pragma unroll
+  for (int i = 0; i < KR; ++i)
+    if (p.active && p.row + i * p.step < t.R) {
+      Packed<T, V> r = {}, o;
+      if (res) r.load(res + first + i * stride);
+      float dz[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        float xh;
+        dz[v] = through(i, v, r.get(v), xh);
+        sz[v] += dz[v];
+        sx[v] += dz[v] * xh;
+      }
+      if (dres) {
+#pragma unroll
+        for (int v = 0; v < V / 2; ++v) o.set2(v, dz[2 * v], dz[2 * v + 1]);
+        o.store(dres + first + i * stride);
+      }
+    }
+  rows_to_waves<V>(sz, t.lanes, p.col / V, part[0]);
+  rows_to_waves<V>(sx, t.lanes, p.col / V, part[1]);
+  __syncthreads();
+  // what the parameters' gradients get of this sample, and back into the first wave's place, times
+  // gamma, for the groups
+  for (int c = threadIdx.x; c < t.groups * t.Cg; c += blockDim.x) {
+    float z = 0.f, xs = 0.f;
+    for (int w = 0; w < waves; ++w) {
+      z += part[0][w * pitch + c];
+      xs += part[1][w * pitch + c];
+    }
+    ws[p.n * t.C + p.c0 + c] = make_float2(z, xs);
+    const float a = load_param(gamma, p.c0 + c, wf, 1.f);
+    part[0][c] = z * a;
+    part[1][c] = xs * a;
+  }
+  if (!dx) return;
+  __syncthreads();
+  const int lane = threadIdx.x & 63;
+  for (int k = threadIdx.x >> 6; k < t.groups; k += waves) {
+    float z = 0.f, xs = 0.f;
+    for (int c = lane; c < t.Cg; c += 64) {
+      z += part[0][k * t.Cg + c];
+      xs += part[1][k * t.Cg + c];
+    }
+    z = wave_sum(z);
+    xs = wave_sum(xs);
+    if (lane == 0) group[0][k] = z, group[1][k] = xs;
+  }
+  __syncthreads();
+  if (!p.active) return;
+  const float inv = 1.f / ((float)t.R * (float)t.Cg);
+  float mz[V], mx[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) mz[v] = group[0][g[v]] * inv, mx[v] = group[1][g[v]] * inv;
+#pragma unroll
+  for (int i = 0; i < KR; ++i)
+    if (p.row + i * p.step < t.R) {
+      Packed<T, V> r = {}, o;
+      if (res) r.load(res + first + i * stride);
+      float d[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        float xh;
+        const float dz = through(i, v, r.get(v), xh);
+        d[v] = rs[v] * (dz * ga[v] - mz[v] - xh * mx[v]);
+      }
+#pragma unroll
+      for (int v = 0; v < V / 2; ++v) o.set2(v, d[2 * v], d[2 * v + 1]);
+      o.store(dx + first + i * stride);
+    }
+}
+
 // ------------------------------------------------------------------ host
 struct Image {
   int64_t N, R;
@@ -414,6 +650,54 @@ Shape shape_of(const Image& im, int64_t groups, int V) {
   return s;
 }
 
+struct Plan {
+  Tile t;
+  int threads = 0, rows = 0;  // threads of a block, rows of a thread; 0: the groups do not fit
+};
+
+// Which groups a block takes: as few idle lanes, as long pieces of memory and as many blocks as go
+// together. 64x64x32x32 in bf16, forward and back with a residual: pieces of 16 bytes PIECE16, 32
+// PIECE32, 64 PIECE64.
+Plan plan_of(const Image& im, int64_t groups, int V, int64_t elem, int max_threads) {
+  Plan best;
+  double least = 1e30;
+  const int G = (int)groups, Cg = im.C / G;
+  if (V * elem < 8) return best;
+  for (int k = 1; k <= G; ++k) {
+    const int c = k * Cg;
+    if (G % k || c % V || c > MAX_CHANNELS || c > 64 * V) continue;
+    int lanes = 0;
+    while ((1 << lanes) * V < c) ++lanes;
+    // four rows a thread keep enough loads on their way; sixteen are what registers hold
+    int threads = 64;
+    while (threads < max_threads && (threads >> lanes) * 4 < im.R) threads *= 2;
+    if ((int64_t)(threads >> lanes) * 16 < im.R) continue;
+    const int64_t blocks = im.N * (G / k);
+    if (blocks >= (1LL << 31)) continue;
+    const double piece = c * elem, idle = (double)(V << lanes) / c;
+    const double cost = idle * (piece >= 128 ? 1.0 : piece >= 64 ? 1.05 : piece >= 32 ? 1.3 : 1.8) *
+                        std::max(1.0, 256.0 / blocks);
+    if (cost < least) {
+      least = cost;
+      best.t = {im.R, im.C, G, Cg, k, lanes, G / k, blocks};
+      best.threads = threads;
+      best.rows = (int64_t)(threads >> lanes) * 4 < im.R ? 16 : 4;
+    }
+  }
+  return best;
+}
+
+// kernels for vectors of 8 bytes and more, 4 or 16 rows a thread
+#define GN_DISPATCH_ROWS(ROWS, ...)                               \
+  if ((ROWS) == 4) { constexpr int KR = 4; __VA_ARGS__; }         \
+  else { constexpr int KR = 16; __VA_ARGS__; }
+#define GN_DISPATCH_TILE(V_VALUE, ROWS, ...)                                                       \
+  switch (V_VALUE) {                                                                               \
+    case 8: { constexpr int V = sizeof(T) == 2 ? 8 : 4; GN_DISPATCH_ROWS(ROWS, __VA_ARGS__) } break; \
+    case 4: { constexpr int V = 4; GN_DISPATCH_ROWS(ROWS, __VA_ARGS__) } break;                    \
+    default: { constexpr int V = sizeof(T) == 2 ? 4 : 2; GN_DISPATCH_ROWS(ROWS, __VA_ARGS__) }      \
+  }
+
 #define GN_DISPATCH_VEC(V_VALUE, ...)                                      \
   switch (V_VALUE) {                                                       \
     case 8: { constexpr int V = sizeof(T) == 2 ? 8 : 4; __VA_ARGS__; } break; \
@@ -437,8 +721,17 @@ void normalise(Forward& f, int64_t groups, double eps, int64_t act) {
   if (x.numel() == 0) return;
   const bool wf = (w.defined() ? w : b.defined() ? b : x).scalar_type() == at::kFloat;
   const int vec = vector_of(im.C, x.element_size(), {ptr(x), ptr(res), ptr(y)});
-  const Shape s = shape_of(im, groups, vec);
   const hipStream_t st = stream_of(x);
+  const Plan plan = plan_of(im, groups, vec, x.element_size(), 1024);
+  if (plan.threads) {
+    MM_DISPATCH_TYPE(x, GN_DISPATCH_TILE(vec, plan.rows, MM_DISPATCH_ACT(act, (
+        gn_tile_kernel<T, V, ACT, KR><<<(unsigned)plan.t.blocks, plan.threads, 0, st>>>(
+            (const T*)ptr(x), (const T*)ptr(res), plan.t, (float)eps, ptr(w), ptr(b), wf,
+            (T*)y.data_ptr(), mean.data_ptr<float>(), rstd.data_ptr<float>())))));
+    check_launch("group_norm_act");
+    return;
+  }
+  const Shape s = shape_of(im, groups, vec);
   Tensor ws = at::empty({im.N * s.S * s.C * 2}, mean.options());
   const unsigned blocks = (unsigned)(im.N * s.tiles * s.S);
   MM_DISPATCH_TYPE(x, GN_DISPATCH_VEC(vec, {
@@ -473,11 +766,24 @@ Grads backward_of(const Tensor& dy, const Tensor& x, int64_t groups, const Tenso
   const bool wf = (w.defined() ? w : b.defined() ? b : x).scalar_type() == at::kFloat;
   const int vec = vector_of(im.C, x.element_size(),
                             {ptr(x), ptr(dy), ptr(res), ptr(g.dx), ptr(g.dres)});
-  const Shape s = shape_of(im, groups, vec);
   const hipStream_t st = stream_of(x);
-  Tensor ws = at::empty({im.N * s.S * s.C * 2}, mean.options());
-  Tensor avg = at::empty({im.N * groups * 2}, mean.options());
-  const unsigned blocks = (unsigned)(im.N * s.tiles * s.S);
+  const Plan plan = plan_of(im, groups, vec, x.element_size(), 512);
+  Tensor ws;
+  int64_t rows;  // of ws: what each sample, or each chunk of it, adds to the parameters' gradients
+  if (plan.threads) {
+    ws = at::empty({im.N * im.C * 2}, mean.options());
+    rows = im.N;
+    MM_DISPATCH_TYPE(x, GN_DISPATCH_TILE(vec, plan.rows, MM_DISPATCH_ACT(act, (
+        gn_tile_bwd_kernel<T, V, ACT, KR><<<(unsigned)plan.t.blocks, plan.threads, 0, st>>>(
+            (const T*)ptr(x), (const T*)ptr(dy), (const T*)ptr(res), plan.t, mean.data_ptr<float>(),
+            rstd.data_ptr<float>(), ptr(w), ptr(b), wf, (T*)ptr(g.dx), (T*)ptr(g.dres),
+            (float2*)ws.data_ptr())))));
+  } else {
+    const Shape s = shape_of(im, groups, vec);
+    ws = at::empty({im.N * s.S * s.C * 2}, mean.options());
+    rows = im.N * s.S;
+    Tensor avg = at::empty({im.N * groups * 2}, mean.options());
+    const unsigned blocks = (unsigned)(im.N * s.tiles * s.S);
   MM_DISPATCH_TYPE(x, GN_DISPATCH_VEC(vec, {
     MM_DISPATCH_ACT(act, (gn_bwd_sums_kernel<T, V, ACT><<<blocks, NT, 0, st>>>(
         (const T*)ptr(x), (const T*)ptr(dy), (const T*)ptr(res), s, mean.data_ptr<float>(),
@@ -491,9 +797,10 @@ Grads backward_of(const Tensor& dy, const Tensor& x, int64_t groups, const Tenso
           (T*)g.dx.data_ptr())));
     }
   }));
+  }
   if (need_dw || need_db)
-    gn_bwd_params_kernel<<<(unsigned)ceil_div(s.C, 64), 1024, 0, st>>>(
-        (const float2*)ws.data_ptr(), im.N * s.S, s.C, wf, (void*)ptr(g.dw), (void*)ptr(g.db));
+    gn_bwd_params_kernel<<<(unsigned)ceil_div(im.C, 64), 1024, 0, st>>>(
+        (const float2*)ws.data_ptr(), rows, im.C, wf, (void*)ptr(g.dw), (void*)ptr(g.db));
   check_launch("group_norm_act backward");
   return g;
 }

@@ -46,6 +46,35 @@ struct alignas(sizeof(T) * V) Vec {
   T e[V];
 };
 
+// V values as they lie in memory, two bf16 a register. (Arrays of 16-bit values take a register
+// each as soon as they are looked at.)
+template <typename T, int V>
+struct Packed {
+  static constexpr int W = V * sizeof(T) / 4;
+  unsigned int w[W];
+  __device__ __forceinline__ void load(const T* p) {
+    *this = *(const Packed*)__builtin_assume_aligned(p, sizeof(T) * V);
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    *(Packed*)__builtin_assume_aligned(p, sizeof(T) * V) = *this;
+  }
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+    else return __uint_as_float(i & 1 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+  }
+  // values 2i and 2i + 1
+  __device__ __forceinline__ void set2(int i, float a, float b) {
+    if constexpr (sizeof(T) == 4) {
+      w[2 * i] = __float_as_uint(a);
+      w[2 * i + 1] = __float_as_uint(b);
+    } else {
+      typedef float f2 __attribute__((ext_vector_type(2)));
+      typedef __bf16 h2 __attribute__((ext_vector_type(2)));
+      w[i] = __builtin_bit_cast(unsigned int, __builtin_convertvector((f2){a, b}, h2));
+    }
+  }
+};
+
 // a parameter that is held in the activations' type or in fp32
 __device__ __forceinline__ float load_param(const void* p, int64_t i, bool is_float, float none) {
   if (p == nullptr) return none;
@@ -67,12 +96,35 @@ __device__ __forceinline__ float wave_sum(float v) {
 // ------------------------------------------------------------- activations
 enum Act { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3 };
 
+// Exponential and reciprocal are the hardware's, within one unit in the last place: an exact
+// division alone would take more instructions than all of the rest.
+__device__ __forceinline__ float exp_neg(float x) {  // exp(-x)
+  return __builtin_amdgcn_exp2f(x * -1.44269504088896341f);
+}
+__device__ __forceinline__ float sigmoid(float z) {
+  return __builtin_amdgcn_rcpf(1.f + exp_neg(z));
+}
+// The normal distribution at z, and exp(-z*z/2), which its density shares with it: erfc by
+// Abramowitz and Stegun, 7.1.26, within 1.5e-7.
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+  const float a = fabsf(z) * 0.70710678118654752f;
+  const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * a);
+  e = exp_neg(a * a);
+  const float poly =
+      t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+  const float half = 0.5f * poly * e;
+  return z < 0.f ? half : 1.f - half;
+}
+
 // act(z). A NaN stays one in each of them.
 template <int ACT>
 __device__ __forceinline__ float act_fwd(float z) {
   if constexpr (ACT == ACT_RELU) return z < 0.f ? 0.f : z;
-  if constexpr (ACT == ACT_SILU) return z / (1.f + __expf(-z));
-  if constexpr (ACT == ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+  if constexpr (ACT == ACT_SILU) return z * sigmoid(z);
+  if constexpr (ACT == ACT_GELU) {
+    float e;
+    return z * normal_cdf(z, e);
+  }
   return z;
 }
 
@@ -81,12 +133,13 @@ template <int ACT>
 __device__ __forceinline__ float act_bwd(float dy, float z) {
   if constexpr (ACT == ACT_RELU) return z <= 0.f ? 0.f : dy;
   if constexpr (ACT == ACT_SILU) {
-    const float s = 1.f / (1.f + __expf(-z));
-    return dy * s * (1.f + z * (1.f - s));
+    const float s = sigmoid(z);
+    return dy * (s * (1.f + z * (1.f - s)));
   }
   if constexpr (ACT == ACT_GELU) {
-    const float cdf = 0.5f * (1.f + erff(z * 0.70710678118654752f));
-    return dy * (cdf + z * (__expf(-0.5f * z * z) * 0.39894228040143268f));
+    float e;
+    const float cdf = normal_cdf(z, e);
+    return dy * (cdf + z * (e * 0.39894228040143268f));
   }
   return dy;
 }
