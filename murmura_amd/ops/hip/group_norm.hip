@@ -59,10 +59,8 @@ __device__ __forceinline__ Place place_of(const Shape& s) {
 // what the waves have, the caller adds them after the barrier.
 template <int V>
 __device__ __forceinline__ void rows_to_waves(float (&acc)[V], int lanes, int col, float* part) {
-  for (int off = 1 << lanes; off < 64; off <<= 1) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) acc[v] += __shfl_xor(acc[v], off, 64);
-  }
+  for (int v = 0; v < V; ++v) acc[v] = lanes_sum(acc[v], lanes);
   const int tile = (1 << lanes) * V;
   if ((threadIdx.x & 63) < (1 << lanes)) {
 #pragma unroll
@@ -354,10 +352,12 @@ struct Tile {
   int lanes;      // log2 of the lanes along the channels, the last of which may be idle
   int tiles;      // of a sample
   int64_t blocks;
+  unsigned int magic;  // for division by Cg
 };
 
 constexpr int MAX_WAVES = 16;
 constexpr int MAX_CHANNELS = 512;
+constexpr int FWD_ROWS = 16, BWD_ROWS = 14;  // of a thread, at most
 
 struct Spot {
   int64_t n;
@@ -380,20 +380,20 @@ __device__ __forceinline__ Spot spot_of(const Tile& t) {
   return p;
 }
 
-// sums of `part` [waves][pitch] over waves and the channels of each group, one wave a group
+// Sums of `part` [waves][pitch] over the waves and the channels of each group: a row of 16 lanes a
+// group, each lane over every 16th of its values.
 __device__ __forceinline__ void over_groups(const float* part, const Tile& t, int pitch, float* to) {
-  const int waves = blockDim.x >> 6, lane = threadIdx.x & 63;
-  for (int g = threadIdx.x >> 6; g < t.groups; g += waves) {
+  const int waves = blockDim.x >> 6, lane = threadIdx.x & 15, entries = waves * t.Cg;
+  for (int g = threadIdx.x >> 4; g < t.groups; g += blockDim.x >> 4) {
     float s = 0.f;
-    for (int c = lane % t.Cg, w = lane / t.Cg, stop = 64 / t.Cg * t.Cg; lane < stop && w < waves;
-         w += 64 / t.Cg)
-      s += part[w * pitch + g * t.Cg + c];
-    if (t.Cg > 64) {
-      s = 0.f;
-      for (int w = 0; w < waves; ++w)
-        for (int c = lane; c < t.Cg; c += 64) s += part[w * pitch + g * t.Cg + c];
+    for (int e = lane; e < entries; e += 16) {
+      const int w = divided(e, t.magic);
+      s += part[w * pitch + g * t.Cg + e - w * t.Cg];
     }
-    s = wave_sum(s);
+    s += moved<0x128>(s);
+    s += moved<0x124>(s);
+    s += moved<0x4E>(s);
+    s += moved<0xB1>(s);
     if (lane == 0) to[g] = s;
   }
 }
@@ -411,12 +411,17 @@ __global__ __launch_bounds__(1024) void gn_tile_kernel(
   const int64_t first = (p.n * t.R + p.row) * t.C + p.c0 + p.col, stride = (int64_t)p.step * t.C;
   int g[V];
 #pragma unroll
-  for (int v = 0; v < V; ++v) g[v] = p.active ? (p.col + v) / t.Cg : 0;
+  for (int v = 0; v < V; ++v) g[v] = p.active ? divided(p.col + v, t.magic) : 0;
   Packed<T, V> val[KR];
-  float acc[V] = {};
+  float acc[V] = {}, ga[V], be[V];
 #pragma unroll
   for (int i = 0; i < KR; ++i)
     if (p.active && p.row + i * p.step < t.R) val[i].load(x + first + i * stride);
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    ga[v] = load_param(gamma, p.c0 + (p.active ? p.col + v : 0), wf, 1.f);
+    be[v] = load_param(beta, p.c0 + (p.active ? p.col + v : 0), wf, 0.f);
+  }
 #pragma unroll
   for (int i = 0; i < KR; ++i)
     if (p.active && p.row + i * p.step < t.R) {
@@ -449,13 +454,8 @@ __global__ __launch_bounds__(1024) void gn_tile_kernel(
     rstd[at] = 1.f / sqrtf(spread[i] * inv + eps);
   }
   if (!p.active) return;
-  float rs[V], ga[V], be[V];
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    rs[v] = 1.f / sqrtf(spread[g[v]] * inv + eps);
-    ga[v] = load_param(gamma, p.c0 + p.col + v, wf, 1.f);
-    be[v] = load_param(beta, p.c0 + p.col + v, wf, 0.f);
-  }
+  for (int v = 0; v < V; ++v) ga[v] *= 1.f / sqrtf(spread[g[v]] * inv + eps);
 #pragma unroll
   for (int i = 0; i < KR; ++i)
     if (p.row + i * p.step < t.R) {
@@ -464,11 +464,50 @@ __global__ __launch_bounds__(1024) void gn_tile_kernel(
       float z[V];
 #pragma unroll
       for (int v = 0; v < V; ++v)
-        z[v] = act_fwd<ACT>((val[i].get(v) - mu[v]) * rs[v] * ga[v] + be[v] + r.get(v));
+        z[v] = act_fwd<ACT>((val[i].get(v) - mu[v]) * ga[v] + be[v] + r.get(v));
 #pragma unroll
       for (int v = 0; v < V / 2; ++v) o.set2(v, z[2 * v], z[2 * v + 1]);
       o.store(y + first + i * stride);
     }
+}
+
+// The block's sums of dz and dz * xhat: to ws, a sample's part of the parameters' gradients, and times
+// gamma over each group to `group`.
+template <int V>
+__device__ __forceinline__ void join_sums(float (&sz)[V], float (&sx)[V], const Tile& t, const Spot& p,
+                                          const void* gamma, bool wf, float* part_z, float* part_x,
+                                          float (*group)[MAX_CHANNELS], float2* ws, bool groups) {
+  const int pitch = V << t.lanes, waves = blockDim.x >> 6;
+  rows_to_waves<V>(sz, t.lanes, p.col / V, part_z);
+  rows_to_waves<V>(sx, t.lanes, p.col / V, part_x);
+  __syncthreads();
+  for (int c = threadIdx.x; c < t.groups * t.Cg; c += blockDim.x) {
+    float z = 0.f, xs = 0.f;
+    for (int w = 0; w < waves; ++w) {
+      z += part_z[w * pitch + c];
+      xs += part_x[w * pitch + c];
+    }
+    ws[p.n * t.C + p.c0 + c] = make_float2(z, xs);
+    const float a = load_param(gamma, p.c0 + c, wf, 1.f);
+    part_z[c] = z * a;  // nobody else reads this place
+    part_x[c] = xs * a;
+  }
+  if (!groups) return;
+  __syncthreads();
+  const int lane = threadIdx.x & 15;
+  for (int k = threadIdx.x >> 4; k < t.groups; k += blockDim.x >> 4) {
+    float z = 0.f, xs = 0.f;
+    for (int c = lane; c < t.Cg; c += 16) {
+      z += part_z[k * t.Cg + c];
+      xs += part_x[k * t.Cg + c];
+    }
+    z += moved<0x128>(z), xs += moved<0x128>(xs);
+    z += moved<0x124>(z), xs += moved<0x124>(xs);
+    z += moved<0x4E>(z), xs += moved<0x4E>(xs);
+    z += moved<0xB1>(z), xs += moved<0xB1>(xs);
+    if (lane == 0) group[0][k] = z, group[1][k] = xs;
+  }
+  __syncthreads();
 }
 
 template <typename T, int V, int ACT, int KR>
@@ -480,20 +519,187 @@ __global__ __launch_bounds__(512) void gn_tile_bwd_kernel(
   __shared__ float part[2][8 * 64 * V];
   __shared__ float group[2][MAX_CHANNELS];
   const Spot p = spot_of<V>(t);
-  const int pitch = V << t.lanes, waves = blockDim.x >> 6;
   const int64_t first = (p.n * t.R + p.row) * t.C + p.c0 + p.col, stride = (int64_t)p.step * t.C;
-  Packed<T, V> xv[KR], dv[KR];
+  // x as it lies in memory, and where dy was, dz in fp32: the activation is gone through once
+  Packed<T, V> xv[KR];
+  float dz[KR][V];
 #pragma unroll
   for (int i = 0; i < KR; ++i)
     if (p.active && p.row + i * p.step < t.R) {
       xv[i].load(x + first + i * stride);
-      dv[i].load(dy + first + i * stride);
+      Packed<T, V> d;
+      d.load(dy + first + i * stride);
+#pragma unroll
+      for (int v = 0; v < V; ++v) dz[i][v] = d.get(v);
     }
+  int g[V];
+  float mu[V], rs[V], ga[V], sz[V] = {}, sx[V] = {};
+  {
+    float be[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      g[v] = p.active ? divided(p.col + v, t.magic) : 0;
+      const int64_t at = p.n * t.G + p.tile * t.groups + g[v];
+      const int c = p.active ? p.c0 + p.col + v : p.c0;
+      mu[v] = mean[at];
+      rs[v] = rstd[at];
+      ga[v] = load_param(gamma, c, wf, 1.f);
+      be[v] = load_param(beta, c, wf, 0.f);
+    }
+#pragma unroll
+    for (int i = 0; i < KR; ++i)
+      if (p.active && p.row + i * p.step < t.R) {
+        Packed<T, V> r = {}, o;
+        if (res) r.load(res + first + i * stride);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float xh = (xv[i].get(v) - mu[v]) * rs[v];
+          dz[i][v] = act_bwd<ACT>(dz[i][v], xh * ga[v] + be[v] + r.get(v));
+          sz[v] += dz[i][v];
+          sx[v] += dz[i][v] * xh;
+        }
+        if (dres) {
+#pragma unroll
+          for (int v = 0; v < V / 2; ++v) o.set2(v, dz[i][2 * v], dz[i][2 * v + 1]);
+          o.store(dres + first + i * stride);
+        }
+      }
+  }
+  join_sums<V>(sz, sx, t, p, gamma, wf, part[0], part[1], group, ws, dx != nullptr);
+  if (!dx || !p.active) return;
+  // dx = rs*ga * dz - rs*rs*avg(dz*ga*xhat) * (x - mu) - rs*avg(dz*ga)
+  const float inv = 1.f / ((float)t.R * (float)t.Cg);
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    sz[v] = rs[v] * (group[0][g[v]] * inv);
+    sx[v] = rs[v] * rs[v] * (group[1][g[v]] * inv);
+    ga[v] *= rs[v];
+  }
+#pragma unroll
+  for (int i = 0; i < KR; ++i)
+    if (p.row + i * p.step < t.R) {
+      Packed<T, V> o;
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        dz[i][v] = dz[i][v] * ga[v] - (xv[i].get(v) - mu[v]) * sx[v] - sz[v];
+#pragma unroll
+      for (int v = 0; v < V / 2; ++v) o.set2(v, dz[i][2 * v], dz[i][2 * v + 1]);
+      o.store(dx + first + i * stride);
+    }
+}
+
+// Groups of more pixels than registers hold: the block goes over its rows twice. A thread's mean and
+// variance grow by four rows at a time, each four around their own mean, and are joined by counts.
+template <typename T, int V, int ACT>
+__global__ __launch_bounds__(512, 4) void gn_stream_kernel(
+    const T* __restrict__ x, const T* __restrict__ res, Tile t, float eps, const void* __restrict__ gamma,
+    const void* __restrict__ beta, bool wf, T* __restrict__ y, float* __restrict__ mean,
+    float* __restrict__ rstd) {
+  constexpr int KR = 4;
+  __shared__ float part[8 * 64 * V];
+  __shared__ float group[MAX_CHANNELS], spread[MAX_CHANNELS];
+  const Spot p = spot_of<V>(t);
+  const int pitch = V << t.lanes;
+  const float inv = 1.f / ((float)t.R * (float)t.Cg);
+  const int64_t first = (p.n * t.R + p.row) * t.C + p.c0 + p.col, stride = (int64_t)p.step * t.C;
+  float mu[V] = {}, m2[V] = {}, seen = 0.f;
+  if (p.active)
+    for (int64_t r = p.row, at = first; r < t.R; r += KR * p.step, at += KR * stride) {
+      Packed<T, V> val[KR];
+#pragma unroll
+      for (int i = 0; i < KR; ++i)
+        if (r + i * p.step < t.R) val[i].load(x + at + i * stride);
+      const float n = (float)min((int64_t)KR, (t.R - r + p.step - 1) / p.step);
+      const float share = 1.f / n, all = 1.f / (seen + n);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        float s = 0.f, q = 0.f;
+#pragma unroll
+        for (int i = 0; i < KR; ++i)
+          if (r + i * p.step < t.R) s += val[i].get(v);
+        s *= share;
+#pragma unroll
+        for (int i = 0; i < KR; ++i)
+          if (r + i * p.step < t.R) {
+            const float d = val[i].get(v) - s;
+            q += d * d;
+          }
+        const float d = s - mu[v];
+        mu[v] += d * (n * all);
+        m2[v] += q + d * d * (seen * n * all);
+      }
+      seen += n;
+    }
+  float acc[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) acc[v] = mu[v] * seen;
+  rows_to_waves<V>(acc, t.lanes, p.col / V, part);
+  __syncthreads();
+  over_groups(part, t, pitch, group);
+  __syncthreads();
+  int g[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    g[v] = p.active ? divided(p.col + v, t.magic) : 0;
+    const float d = mu[v] - group[g[v]] * inv;
+    acc[v] = m2[v] + d * d * seen;
+  }
+  rows_to_waves<V>(acc, t.lanes, p.col / V, part);
+  __syncthreads();
+  over_groups(part, t, pitch, spread);
+  __syncthreads();
+  for (int i = threadIdx.x; i < t.groups; i += blockDim.x) {
+    const int64_t at = p.n * t.G + p.tile * t.groups + i;
+    mean[at] = group[i] * inv;
+    rstd[at] = 1.f / sqrtf(spread[i] * inv + eps);
+  }
+  if (!p.active) return;
+  float be[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    mu[v] = group[g[v]] * inv;
+    m2[v] = load_param(gamma, p.c0 + p.col + v, wf, 1.f) / sqrtf(spread[g[v]] * inv + eps);
+    be[v] = load_param(beta, p.c0 + p.col + v, wf, 0.f);
+  }
+  for (int64_t r = p.row, at = first; r < t.R; r += KR * p.step, at += KR * stride) {
+    Packed<T, V> val[KR], rv[KR] = {};
+#pragma unroll
+    for (int i = 0; i < KR; ++i)
+      if (r + i * p.step < t.R) {
+        val[i].load(x + at + i * stride);
+        if (res) rv[i].load(res + at + i * stride);
+      }
+#pragma unroll
+    for (int i = 0; i < KR; ++i)
+      if (r + i * p.step < t.R) {
+        float z[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          z[v] = act_fwd<ACT>((val[i].get(v) - mu[v]) * m2[v] + be[v] + rv[i].get(v));
+#pragma unroll
+        for (int v = 0; v < V / 2; ++v) val[i].set2(v, z[2 * v], z[2 * v + 1]);
+        val[i].store(y + at + i * stride);
+      }
+  }
+}
+
+// And back: the sums, then dx, the second time while the caches still have some of the rows.
+template <typename T, int V, int ACT>
+__global__ __launch_bounds__(512, 4) void gn_stream_bwd_kernel(
+    const T* __restrict__ x, const T* __restrict__ dy, const T* __restrict__ res, Tile t,
+    const float* __restrict__ mean, const float* __restrict__ rstd, const void* __restrict__ gamma,
+    const void* __restrict__ beta, bool wf, T* __restrict__ dx, T* __restrict__ dres,
+    float2* __restrict__ ws) {
+  constexpr int KR = 2;
+  __shared__ float part[2][8 * 64 * V];
+  __shared__ float group[2][MAX_CHANNELS];
+  const Spot p = spot_of<V>(t);
+  const int64_t first = (p.n * t.R + p.row) * t.C + p.c0 + p.col, stride = (int64_t)p.step * t.C;
   int g[V];
   float mu[V], rs[V], ga[V], be[V], sz[V] = {}, sx[V] = {};
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    g[v] = p.active ? (p.col + v) / t.Cg : 0;
+    g[v] = p.active ? divided(p.col + v, t.magic) : 0;
     const int64_t at = p.n * t.G + p.tile * t.groups + g[v];
     const int c = p.active ? p.c0 + p.col + v : p.c0;
     mu[v] = mean[at];
@@ -501,81 +707,61 @@ __global__ __launch_bounds__(512) void gn_tile_bwd_kernel(
     ga[v] = load_param(gamma, c, wf, 1.f);
     be[v] = load_param(beta, c, wf, 0.f);
   }
-  // dz of a value, from what the registers hold
-  const auto through = [&](int i, int v, float r, float& xh) {
-    xh = (xv[i].get(v) - mu[v]) * rs[v];
-    return act_bwd<ACT>(dv[i].get(v), xh * ga[v] + be[v] + r);
+  // `with` gets each vector's place, xhat and dz
+  const auto rows = [&](auto with) {
+    if (!p.active) return;
+    for (int64_t r = p.row, at = first; r < t.R; r += KR * p.step, at += KR * stride) {
+      Packed<T, V> xv[KR], dv[KR], rv[KR] = {};
+#pragma unroll
+      for (int i = 0; i < KR; ++i)
+        if (r + i * p.step < t.R) {
+          xv[i].load(x + at + i * stride);
+          dv[i].load(dy + at + i * stride);
+          if (res) rv[i].load(res + at + i * stride);
+        }
+#pragma unroll
+      for (int i = 0; i < KR; ++i)
+        if (r + i * p.step < t.R) {
+          float xh[V], dz[V];
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            xh[v] = (xv[i].get(v) - mu[v]) * rs[v];
+            dz[v] = act_bwd<ACT>(dv[i].get(v), xh[v] * ga[v] + be[v] + rv[i].get(v));
+          }
+          with(at + i * stride, xh, dz);
+        }
+    }
   };
+  rows([&](int64_t at, const float (&xh)[V], const float (&dz)[V]) {
 #pragma unroll
-  for (int i = 0; i < KR; ++i)
-    if (p.active && p.row + i * p.step < t.R) {
-      Packed<T, V> r = {}, o;
-      if (res) r.load(res + first + i * stride);
-      float dz[V];
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float xh;
-        dz[v] = through(i, v, r.get(v), xh);
-        sz[v] += dz[v];
-        sx[v] += dz[v] * xh;
-      }
-      if (dres) {
-#pragma unroll
-        for (int v = 0; v < V / 2; ++v) o.set2(v, dz[2 * v], dz[2 * v + 1]);
-        o.store(dres + first + i * stride);
-      }
+    for (int v = 0; v < V; ++v) {
+      sz[v] += dz[v];
+      sx[v] += dz[v] * xh[v];
     }
-  rows_to_waves<V>(sz, t.lanes, p.col / V, part[0]);
-  rows_to_waves<V>(sx, t.lanes, p.col / V, part[1]);
-  __syncthreads();
-  // what the parameters' gradients get of this sample, and back into the first wave's place, times
-  // gamma, for the groups
-  for (int c = threadIdx.x; c < t.groups * t.Cg; c += blockDim.x) {
-    float z = 0.f, xs = 0.f;
-    for (int w = 0; w < waves; ++w) {
-      z += part[0][w * pitch + c];
-      xs += part[1][w * pitch + c];
+    if (dres) {
+      Packed<T, V> o;
+#pragma unroll
+      for (int v = 0; v < V / 2; ++v) o.set2(v, dz[2 * v], dz[2 * v + 1]);
+      o.store(dres + at);
     }
-    ws[p.n * t.C + p.c0 + c] = make_float2(z, xs);
-    const float a = load_param(gamma, p.c0 + c, wf, 1.f);
-    part[0][c] = z * a;
-    part[1][c] = xs * a;
-  }
+  });
+  join_sums<V>(sz, sx, t, p, gamma, wf, part[0], part[1], group, ws, dx != nullptr);
   if (!dx) return;
-  __syncthreads();
-  const int lane = threadIdx.x & 63;
-  for (int k = threadIdx.x >> 6; k < t.groups; k += waves) {
-    float z = 0.f, xs = 0.f;
-    for (int c = lane; c < t.Cg; c += 64) {
-      z += part[0][k * t.Cg + c];
-      xs += part[1][k * t.Cg + c];
-    }
-    z = wave_sum(z);
-    xs = wave_sum(xs);
-    if (lane == 0) group[0][k] = z, group[1][k] = xs;
-  }
-  __syncthreads();
-  if (!p.active) return;
   const float inv = 1.f / ((float)t.R * (float)t.Cg);
-  float mz[V], mx[V];
 #pragma unroll
-  for (int v = 0; v < V; ++v) mz[v] = group[0][g[v]] * inv, mx[v] = group[1][g[v]] * inv;
+  for (int v = 0; v < V; ++v) {
+    sz[v] = group[0][g[v]] * inv;
+    sx[v] = group[1][g[v]] * inv;
+  }
+  rows([&](int64_t at, const float (&xh)[V], const float (&dz)[V]) {
+    Packed<T, V> o;
+    float d[V];
 #pragma unroll
-  for (int i = 0; i < KR; ++i)
-    if (p.row + i * p.step < t.R) {
-      Packed<T, V> r = {}, o;
-      if (res) r.load(res + first + i * stride);
-      float d[V];
+    for (int v = 0; v < V; ++v) d[v] = rs[v] * (dz[v] * ga[v] - sz[v] - xh[v] * sx[v]);
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float xh;
-        const float dz = through(i, v, r.get(v), xh);
-        d[v] = rs[v] * (dz * ga[v] - mz[v] - xh * mx[v]);
-      }
-#pragma unroll
-      for (int v = 0; v < V / 2; ++v) o.set2(v, d[2 * v], d[2 * v + 1]);
-      o.store(dx + first + i * stride);
-    }
+    for (int v = 0; v < V / 2; ++v) o.set2(v, d[2 * v], d[2 * v + 1]);
+    o.store(dx + at);
+  });
 }
 
 // ------------------------------------------------------------------ host
@@ -652,13 +838,18 @@ Shape shape_of(const Image& im, int64_t groups, int V) {
 
 struct Plan {
   Tile t;
-  int threads = 0, rows = 0;  // threads of a block, rows of a thread; 0: the groups do not fit
+  int threads = 0;  // of a block; 0: chunks of rows for many blocks, statistics joined between kernels
+  int rows = 0;     // of a thread; 0: any number, read twice
 };
 
-// Which groups a block takes: as few idle lanes, as long pieces of memory and as many blocks as go
-// together. 64x64x32x32 in bf16, forward and back with a residual: pieces of 16 bytes PIECE16, 32
-// PIECE32, 64 PIECE64.
-Plan plan_of(const Image& im, int64_t groups, int V, int64_t elem, int max_threads) {
+// Which groups a block takes, and whether it holds their pixels: as few idle lanes, as long pieces of
+// memory and as many blocks as go together, by the penalties below. Measured, going back:
+// 128x256x56x56 in bf16 250 us held, in pieces of 32 bytes, and 233 and 220 read twice in 128 and 256;
+// 128x128x112x112 830 us by chunks, 600, 491 and 425 read twice in pieces of 32, 64 and 128;
+// 64x256x28x28 33 us held in 128, 53 read twice. Forward, 64x64x32x32: 11.4 us in pieces of 32 bytes
+// and 256 blocks, 13.5 in 16 and 512, 12.8 in 64 and 128; 128x256x56x56 141 held in 64, 198 in 32.
+Plan plan_of(const Image& im, int64_t groups, int V, int64_t elem, int max_threads, int most,
+             double twice) {
   Plan best;
   double least = 1e30;
   const int G = (int)groups, Cg = im.C / G;
@@ -668,35 +859,50 @@ Plan plan_of(const Image& im, int64_t groups, int V, int64_t elem, int max_threa
     if (G % k || c % V || c > MAX_CHANNELS || c > 64 * V) continue;
     int lanes = 0;
     while ((1 << lanes) * V < c) ++lanes;
-    // four rows a thread keep enough loads on their way; sixteen are what registers hold
-    int threads = 64;
-    while (threads < max_threads && (threads >> lanes) * 4 < im.R) threads *= 2;
-    if ((int64_t)(threads >> lanes) * 16 < im.R) continue;
     const int64_t blocks = im.N * (G / k);
     if (blocks >= (1LL << 31)) continue;
+    // four rows a thread keep enough loads on their way; `most` are what registers hold
+    int threads = 64;
+    while (threads < max_threads && (threads >> lanes) * 4 < im.R) threads *= 2;
+    int rows = (int64_t)(threads >> lanes) * 4 >= im.R ? 4 : (int64_t)(threads >> lanes) * most >= im.R ? most : 0;
     const double piece = c * elem, idle = (double)(V << lanes) / c;
     const double cost = idle * (piece >= 128 ? 1.0 : piece >= 64 ? 1.05 : piece >= 32 ? 1.3 : 1.8) *
-                        std::max(1.0, 256.0 / blocks);
+                        std::max(1.0, 256.0 / blocks) * (rows ? 1.0 : twice);
     if (cost < least) {
       least = cost;
-      best.t = {im.R, im.C, G, Cg, k, lanes, G / k, blocks};
-      best.threads = threads;
-      best.rows = (int64_t)(threads >> lanes) * 4 < im.R ? 16 : 4;
+      best.t = {im.R, im.C, G, Cg, k, lanes, G / k, blocks, magic_of(Cg)};
+      best.threads = rows ? threads : 512;
+      best.rows = rows;
     }
   }
+  // few blocks with much to read: one image of 64x256x256 in bf16 would be 8 blocks of a megabyte
+  if (best.threads && best.t.blocks < 128 && im.N * im.R * im.C * elem / best.t.blocks > (256 << 10))
+    best.threads = 0;
   return best;
 }
 
 // kernels for vectors of 8 bytes and more, 4 or 16 rows a thread
-#define GN_DISPATCH_ROWS(ROWS, ...)                               \
+#define GN_DISPATCH_ROWS(ROWS, MOST, ...)                         \
   if ((ROWS) == 4) { constexpr int KR = 4; __VA_ARGS__; }         \
-  else { constexpr int KR = 16; __VA_ARGS__; }
-#define GN_DISPATCH_TILE(V_VALUE, ROWS, ...)                                                       \
-  switch (V_VALUE) {                                                                               \
-    case 8: { constexpr int V = sizeof(T) == 2 ? 8 : 4; GN_DISPATCH_ROWS(ROWS, __VA_ARGS__) } break; \
-    case 4: { constexpr int V = 4; GN_DISPATCH_ROWS(ROWS, __VA_ARGS__) } break;                    \
-    default: { constexpr int V = sizeof(T) == 2 ? 4 : 2; GN_DISPATCH_ROWS(ROWS, __VA_ARGS__) }      \
+  else if ((ROWS) == (MOST)) { constexpr int KR = MOST; __VA_ARGS__; } \
+  else { constexpr int KR = 0; __VA_ARGS__; }
+#define GN_DISPATCH_TILE(V_VALUE, ROWS, MOST, ...)                                                       \
+  switch (V_VALUE) {                                                                                     \
+    case 8: { constexpr int V = sizeof(T) == 2 ? 8 : 4; GN_DISPATCH_ROWS(ROWS, MOST, __VA_ARGS__) } break; \
+    case 4: { constexpr int V = 4; GN_DISPATCH_ROWS(ROWS, MOST, __VA_ARGS__) } break;                    \
+    default: { constexpr int V = sizeof(T) == 2 ? 4 : 2; GN_DISPATCH_ROWS(ROWS, MOST, __VA_ARGS__) }      \
   }
+
+template <typename T, int V, int ACT, int KR>
+auto tile_of() {
+  if constexpr (KR) return &gn_tile_kernel<T, V, ACT, KR>;
+  else return &gn_stream_kernel<T, V, ACT>;
+}
+template <typename T, int V, int ACT, int KR>
+auto tile_bwd_of() {
+  if constexpr (KR) return &gn_tile_bwd_kernel<T, V, ACT, KR>;
+  else return &gn_stream_bwd_kernel<T, V, ACT>;
+}
 
 #define GN_DISPATCH_VEC(V_VALUE, ...)                                      \
   switch (V_VALUE) {                                                       \
@@ -722,10 +928,10 @@ void normalise(Forward& f, int64_t groups, double eps, int64_t act) {
   const bool wf = (w.defined() ? w : b.defined() ? b : x).scalar_type() == at::kFloat;
   const int vec = vector_of(im.C, x.element_size(), {ptr(x), ptr(res), ptr(y)});
   const hipStream_t st = stream_of(x);
-  const Plan plan = plan_of(im, groups, vec, x.element_size(), 1024);
+  const Plan plan = plan_of(im, groups, vec, x.element_size(), 1024, FWD_ROWS, 1.5);
   if (plan.threads) {
-    MM_DISPATCH_TYPE(x, GN_DISPATCH_TILE(vec, plan.rows, MM_DISPATCH_ACT(act, (
-        gn_tile_kernel<T, V, ACT, KR><<<(unsigned)plan.t.blocks, plan.threads, 0, st>>>(
+    MM_DISPATCH_TYPE(x, GN_DISPATCH_TILE(vec, plan.rows, FWD_ROWS, MM_DISPATCH_ACT(act, (
+        tile_of<T, V, ACT, KR>()<<<(unsigned)plan.t.blocks, plan.threads, 0, st>>>(
             (const T*)ptr(x), (const T*)ptr(res), plan.t, (float)eps, ptr(w), ptr(b), wf,
             (T*)y.data_ptr(), mean.data_ptr<float>(), rstd.data_ptr<float>())))));
     check_launch("group_norm_act");
@@ -767,14 +973,14 @@ Grads backward_of(const Tensor& dy, const Tensor& x, int64_t groups, const Tenso
   const int vec = vector_of(im.C, x.element_size(),
                             {ptr(x), ptr(dy), ptr(res), ptr(g.dx), ptr(g.dres)});
   const hipStream_t st = stream_of(x);
-  const Plan plan = plan_of(im, groups, vec, x.element_size(), 512);
+  const Plan plan = plan_of(im, groups, vec, x.element_size(), 512, BWD_ROWS, 1.15);
   Tensor ws;
   int64_t rows;  // of ws: what each sample, or each chunk of it, adds to the parameters' gradients
   if (plan.threads) {
     ws = at::empty({im.N * im.C * 2}, mean.options());
     rows = im.N;
-    MM_DISPATCH_TYPE(x, GN_DISPATCH_TILE(vec, plan.rows, MM_DISPATCH_ACT(act, (
-        gn_tile_bwd_kernel<T, V, ACT, KR><<<(unsigned)plan.t.blocks, plan.threads, 0, st>>>(
+    MM_DISPATCH_TYPE(x, GN_DISPATCH_TILE(vec, plan.rows, BWD_ROWS, MM_DISPATCH_ACT(act, (
+        tile_bwd_of<T, V, ACT, KR>()<<<(unsigned)plan.t.blocks, plan.threads, 0, st>>>(
             (const T*)ptr(x), (const T*)ptr(dy), (const T*)ptr(res), plan.t, mean.data_ptr<float>(),
             rstd.data_ptr<float>(), ptr(w), ptr(b), wf, (T*)ptr(g.dx), (T*)ptr(g.dres),
             (float2*)ws.data_ptr())))));

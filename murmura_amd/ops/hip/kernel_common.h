@@ -87,10 +87,36 @@ __device__ __forceinline__ void store_param(void* p, int64_t i, bool is_float, f
     ((bf16*)p)[i] = round_bf16(v);
 }
 
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+// v of the lane that is `DPP`'s move away
+template <int DPP>
+__device__ __forceinline__ float moved(float v) {
+  return __uint_as_float((unsigned int)__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), DPP, 0xF, 0xF, true));
+}
+
+// Sum over the lanes that are alike in the low log2 `lanes` bits of their number, in all of them:
+// rows of 16 by the adder's own lane moves (turned by 8 and 4, then within quads), rows by swapping
+// them.
+__device__ __forceinline__ float lanes_sum(float v, int lanes) {
+  if (lanes < 4) v += moved<0x128>(v);  // turned by 8
+  if (lanes < 3) v += moved<0x124>(v);  // by 4
+  if (lanes < 2) v += moved<0x4E>(v);   // 2 3 0 1
+  if (lanes < 1) v += moved<0xB1>(v);   // 1 0 3 2
+  if (lanes < 5) {
+    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+  }
+  if (lanes < 6) {
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+  }
   return v;
+}
+
+__device__ __forceinline__ float wave_sum(float v) { return lanes_sum(v, 0); }
+
+// a / d for a < 2^16 and 0 < d < 2^16, by ceil(2^32 / d) (0 stands for 2^32)
+__device__ __forceinline__ int divided(int a, unsigned int magic) {
+  return magic ? (int)__umulhi((unsigned int)a, magic) : a;
 }
 
 // ------------------------------------------------------------- activations
@@ -151,6 +177,10 @@ inline hipStream_t stream_of(const Tensor& t) {
 
 inline bool is_float_type(const Tensor& t) {
   return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16;
+}
+
+inline unsigned int magic_of(int64_t d) {
+  return (unsigned int)(((1LL << 32) + d - 1) / d);  // d = 1 gives 0
 }
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }

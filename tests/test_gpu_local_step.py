@@ -109,7 +109,8 @@ def _gn_check(x, groups, w, b, act, res, dy, eps=1e-5, run=None):
 GN_SHAPES = [
     ((2, 64, 8, 8), 32), ((3, 60, 7, 5), 5), ((1, 6, 1, 1), 3), ((5, 7, 3, 3), 7), ((2, 1030, 4, 4), 1),
     ((2, 36, 33, 31), 9), ((4, 24), 3), ((3, 5), 5), ((1, 8, 70, 70), 2), ((2, 512, 9, 9), 16),
-    ((1, 3, 64, 64), 1), ((2, 96, 40, 3), 2), ((2, 12, 1, 300), 12),
+    ((1, 3, 64, 64), 1), ((2, 96, 40, 3), 2), ((2, 12, 1, 300), 12), ((1, 64, 150, 140), 8), ((9, 32, 70, 75), 2),
+    ((130, 8, 130, 131), 2), ((3, 640, 6, 6), 8), ((1, 1600, 5, 5), 1),
 ]
 
 
