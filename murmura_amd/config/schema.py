@@ -8,7 +8,7 @@ compute dtype). ``extra="forbid"`` everywhere, like the reference.
 
 from __future__ import annotations
 
-from typing import Any, Dict, Literal, Optional
+from typing import Any, Dict, Literal, Optional, Tuple
 
 from pydantic import BaseModel, ConfigDict, Field, model_validator
 
@@ -53,6 +53,19 @@ class TrainingConfig(_Strict):
     batch_size: int = 64
     lr: float = 0.01
     max_samples: Optional[int] = None
+    # MI355X-native additions: the local optimizer. "adamw" keeps its moments
+    # on the node's device, in 32 bits or in 8 (2 bytes a parameter for both)
+    optimizer: Literal["sgd", "adamw"] = "sgd"
+    weight_decay: float = 0.01  # adamw only, as the three below
+    betas: Tuple[float, float] = (0.9, 0.999)
+    eps: float = 1e-8
+    optimizer_bits: Literal[8, 32] = 32
+
+    @model_validator(mode="after")
+    def _betas_below_one(self) -> "TrainingConfig":
+        if not all(0.0 <= b < 1.0 for b in self.betas):
+            raise ValueError("training.betas must lie in [0, 1)")
+        return self
 
 
 class DataConfig(_Strict):

@@ -115,7 +115,12 @@ class TrainGraph:
         params = self._params
         grads = torch.autograd.grad(loss, params)
         with torch.no_grad():
-            torch._foreach_add_(params, grads, alpha=-self._captured_lr)
+            if node.optimizer is not None:
+                # one launch over all tensors; moments and the count of steps
+                # live on the device, so replays go on where the last one ended
+                node.optimizer.step(grads, self._captured_lr)
+            else:
+                torch._foreach_add_(params, grads, alpha=-self._captured_lr)
         self.loss_sum += loss.detach()
 
     def _capture(self) -> None:
@@ -126,6 +131,8 @@ class TrainGraph:
         # warmup on a side stream executes real steps — snapshot/restore the
         # flat state so capture-time warmup does not perturb training
         saved = node.store.flat.clone()
+        states = node.optimizer.tensors() if node.optimizer is not None else []
+        saved_states = [t.clone() for t in states]
         # num_batches_tracked increments are deferred out of the graph (a
         # ~5 us device add per BN per step); local_train bumps them host-side
         # per epoch instead (ops/fused_bn.py bump_num_batches_tracked)
@@ -140,6 +147,8 @@ class TrainGraph:
                     self._one_step(0)
             torch.cuda.current_stream().wait_stream(s)
             node.store.flat.copy_(saved)
+            for t, kept in zip(states, saved_states):
+                t.copy_(kept)
             node.store.zero_grad()
             g = torch.cuda.CUDAGraph()
             with torch.cuda.graph(g):

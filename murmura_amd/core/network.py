@@ -198,7 +198,7 @@ class Network:
         from torch.utils.data import DataLoader
 
         from murmura_amd.utils.device import get_device
-        from murmura_amd.utils.factories import build_attack
+        from murmura_amd.utils.factories import build_attack, build_optimizer
 
         n = config.topology.num_nodes
         topo = create_topology(
@@ -257,6 +257,7 @@ class Network:
                     dtype=dtype,
                     model_factory=model_factory,
                     channels_last=channels_last,
+                    optimizer=build_optimizer(config, i),
                 )
             )
         return cls(nodes, topo, attack=attack, mobility=mobility)

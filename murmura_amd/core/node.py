@@ -23,6 +23,7 @@ from torch import Tensor, nn
 from murmura_amd import ops
 from murmura_amd.aggregation.base import Aggregator, EvalContext
 from murmura_amd.core.flat import FlatParamStore
+from murmura_amd.core.optim import AdamWConfig, NodeAdamW
 from murmura_amd.models.evidential import EvidentialLoss
 from murmura_amd.utils.metrics import evaluate_evidential, evaluate_model
 
@@ -41,6 +42,7 @@ class Node:
         dtype: torch.dtype = torch.float32,
         model_factory: Optional[Callable[[], nn.Module]] = None,
         channels_last: bool = True,
+        optimizer: Optional[AdamWConfig] = None,
     ) -> None:
         self.node_id = node_id
         self.device = torch.device(device)
@@ -53,6 +55,12 @@ class Node:
         )
         self.store = FlatParamStore(model, self.device, dtype, channels_last=self.channels_last)
         self.model = self.store.model
+        # None: plain SGD over the flat prefix
+        self.optimizer: Optional[NodeAdamW] = None
+        if optimizer is not None:
+            self.optimizer = NodeAdamW(
+                [p for p in self.model.parameters() if p.requires_grad], optimizer
+            )
         self.train_loader = train_loader
         self.test_loader = test_loader
         self.aggregator = aggregator
@@ -92,7 +100,7 @@ class Node:
     def local_train(
         self, epochs: int = 1, lr: float = 0.01, round_num: int = 0
     ) -> Dict[str, float]:
-        """Local SGD epochs. Skips batches with < 2 samples (BatchNorm needs
+        """Local epochs of SGD, or of AdamW where the node has one. Skips batches with < 2 samples (BatchNorm needs
         batch > 1 in training mode — reference: node.py:81).
 
         On GPU with a plain CE criterion the whole epoch runs as ONE hipGraph
@@ -139,7 +147,12 @@ class Node:
                 else:
                     loss = self.criterion(out.float(), y)
                 loss.backward()
-                ops.sgd_step(pflat, gflat, lr)
+                if self.optimizer is not None:
+                    self.optimizer.step(
+                        [p.grad for p in self.model.parameters() if p.requires_grad], lr
+                    )
+                else:
+                    ops.sgd_step(pflat, gflat, lr)
                 total_loss = total_loss + loss.detach()
                 num_batches += 1
         mean = (total_loss / max(1, num_batches)).item() if num_batches else 0.0

@@ -455,6 +455,9 @@ void adamw_step(const std::vector<Tensor>& params, std::vector<Tensor> grads,
                 "adamw_step: parameters share memory: pass each once");
   check_state(exp_avg, P, dev);
   check_state(exp_avg_sq, P, dev);
+  // a graph that saved a parameter must not be gone back through with its new values
+  for (const Tensor& p : params)
+    if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
   TORCH_CHECK(exp_avg.size() == exp_avg_sq.size(), "adamw_step: both moments in the same bits");
   TORCH_CHECK(step.device() == dev && step.scalar_type() == at::kLong && step.numel() == 1,
               "adamw_step: step is one int64 on the parameters' device");

@@ -239,11 +239,11 @@ def group_norm_act(x: Tensor, num_groups: int, weight: Optional[Tensor] = None,
     check_group_norm_act(x, num_groups, weight, bias, res)
     check_act(act)
     n, c = x.shape[:2]
-    g = _wide(x).reshape(n, num_groups, -1)
-    if g.shape[2] and n:
+    z = _wide(x)
+    if x.numel():
+        g = z.reshape(n, num_groups, -1)
         d = g - g.mean(2, keepdim=True)
-        g = d / torch.sqrt(d.square().mean(2, keepdim=True) + eps)
-    z = g.reshape(x.shape)
+        z = (d / torch.sqrt(d.square().mean(2, keepdim=True) + eps)).reshape(x.shape)
     per_channel = (1, c) + (1,) * (x.dim() - 2)
     if weight is not None:
         z = z * _wide(weight).view(per_channel)

@@ -114,6 +114,7 @@ def build_node(config: Config, rank: int, device: torch.device) -> Node:
         dtype=dtype,
         model_factory=model_factory,
         channels_last=config.compute.channels_last,
+        optimizer=factories.build_optimizer(config, rank),
     )
 
 

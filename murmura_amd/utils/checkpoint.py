@@ -8,7 +8,8 @@ Format (torch.save):
   {"round": int, "history": dict,
    "nodes": {node_id: {"flat": cpu tensor [P],
                         "nonfloat": {name: tensor},
-                        "dtype": str}}}
+                        "dtype": str,
+                        "optimizer": {"bits": int, "tensors": list}  (AdamW only)}}}
 """
 
 from __future__ import annotations
@@ -25,11 +26,14 @@ def node_state_payload(node) -> dict:
         for name, b in node.model.named_buffers()
         if not torch.is_floating_point(b)
     }
-    return {
+    payload = {
         "flat": node.store.flat.detach().float().cpu().clone(),
         "nonfloat": nonfloat,
         "dtype": str(node.dtype),
     }
+    if getattr(node, "optimizer", None) is not None:
+        payload["optimizer"] = node.optimizer.state_payload()
+    return payload
 
 
 def restore_node_state(node, payload: dict) -> None:
@@ -38,6 +42,9 @@ def restore_node_state(node, payload: dict) -> None:
     for name, val in payload.get("nonfloat", {}).items():
         if name in buffers:
             buffers[name].copy_(val.to(buffers[name].device))
+    # a checkpoint of an SGD run leaves a new optimizer's moments at zero
+    if getattr(node, "optimizer", None) is not None and "optimizer" in payload:
+        node.optimizer.load_payload(payload["optimizer"])
 
 
 def save_checkpoint(path, round_num: int, nodes, history: Optional[dict] = None) -> None:

@@ -23,6 +23,7 @@ from murmura_amd.attacks import (
 )
 from murmura_amd.config.schema import Config
 from murmura_amd.core.flat import calculate_model_dimension
+from murmura_amd.core.optim import AdamWConfig
 from murmura_amd.models import get_evidential_loss
 from murmura_amd.models.zoo import MODEL_FACTORIES
 from murmura_amd.topology.dynamic import MobilityModel
@@ -188,6 +189,16 @@ def build_mobility_model(config: Config) -> Optional[MobilityModel]:
         seed=m.seed,
         ensure_connected=m.ensure_connected,
     )
+
+
+def build_optimizer(config: Config, node_id: int) -> Optional[AdamWConfig]:
+    """training.optimizer -> a node's AdamW settings; None for SGD. Nodes round
+    with seeds of their own."""
+    t = config.training
+    if t.optimizer == "sgd":
+        return None
+    return AdamWConfig(betas=tuple(t.betas), eps=t.eps, weight_decay=t.weight_decay,
+                       state_bits=t.optimizer_bits, seed=config.experiment.seed + node_id)
 
 
 def compute_dtype(config: Config) -> torch.dtype:

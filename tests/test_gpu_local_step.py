@@ -566,3 +566,62 @@ def test_adamw_refusals():
         many = torch.zeros(400, device="cuda")
         ops.adamw_step(list(many.split(1)), list(torch.zeros(400, device="cuda").split(1)), *ops.adamw_state(400, "cuda", 8), 1e-3)
     assert int(t) == 0 and not p.any()
+
+
+# ----------------------------------------------------- a node's whole round
+def _gpu_node(model, optimizer, dtype=BF16, shape=(3, 16, 16), n=48):
+    from torch.utils.data import DataLoader, TensorDataset
+
+    from murmura_amd.aggregation.fedavg import FedAvgAggregator
+    from murmura_amd.core.node import Node
+
+    data = TensorDataset(_randn((n, *shape), FP32, 9), torch.arange(n) % 4)
+    loader = DataLoader(data, batch_size=16)
+    return Node(0, model, loader, loader, FedAvgAggregator(), torch.device("cuda"), dtype=dtype,
+                optimizer=optimizer)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_node_rounds_with_group_norm_and_adamw(bits):
+    from murmura_amd.core.optim import AdamWConfig
+    from murmura_amd.models import ResNet18
+
+    def train():
+        torch.manual_seed(0)
+        node = _gpu_node(ResNet18(num_classes=4, norm="group"), AdamWConfig(state_bits=bits))
+        for r in range(3):  # captured once, replayed, between them a state from outside
+            out = node.local_train(lr=1e-3, round_num=r)
+            assert math.isfinite(out["loss"])
+            node.set_state(node.get_state() * 0.99)
+        assert int(node.optimizer.count) == 9  # warm-up steps are taken back
+        return node
+
+    a = train()
+    assert torch.isfinite(a.get_state()).all()
+    m = a.optimizer.tensors()[0]
+    assert m.count_nonzero() > 0.5 * m.numel()
+
+
+def test_graph_and_eager_node_take_the_same_steps(monkeypatch):
+    """Fused MLP, AdamW in 32 bits: the captured epoch does what single steps do."""
+    from murmura_amd.core.optim import AdamWConfig
+    from murmura_amd.models import SimpleMLP
+
+    def train(graphs):
+        if not graphs:
+            monkeypatch.setenv("MURMURA_NO_GRAPHS", "1")
+        torch.manual_seed(0)
+        node = _gpu_node(SimpleMLP(24, 64, 4, fused=True), AdamWConfig(), dtype=FP32, shape=(24,), n=16)
+        for _ in range(4):
+            node.local_train(lr=1e-2)  # one batch an epoch: its order does not matter to a sum
+        monkeypatch.delenv("MURMURA_NO_GRAPHS", raising=False)
+        return node
+
+    a, b = train(True), train(False)
+    assert int(a.optimizer.count) == int(b.optimizer.count) == 4
+    # The captured epoch sums its 16 samples in another order: gradients differ by 16 * 24 U of
+    # their magnitude. Adam divides by that magnitude, so 4 steps of 1e-2 differ by that share of
+    # themselves, and by twice a whole step where a gradient is all rounding.
+    diff = (a.get_state() - b.get_state()).abs()
+    assert diff.max() <= 4 * 2 * 1e-2
+    assert (diff > 4 * 1e-2 * 16 * 24 * U * 64).float().mean() < 0.02

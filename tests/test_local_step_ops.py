@@ -1,0 +1,241 @@
+"""The local training step's operators on the CPU: their definitions against
+64 bits and differences, their refusals, and the paths that reach them
+(models, configuration, nodes, checkpoints)."""
+
+import math
+
+import pytest
+import torch
+from torch.utils.data import DataLoader, TensorDataset
+
+from murmura_amd import ops
+from murmura_amd.aggregation.fedavg import FedAvgAggregator
+from murmura_amd.config.schema import Config
+from murmura_amd.core.node import Node
+from murmura_amd.core.optim import AdamWConfig
+from murmura_amd.models import FEMNISTModel, ResNet18, SimpleMLP
+from murmura_amd.models.zoo import WideMLP
+from murmura_amd.ops import reference as ref
+from murmura_amd.ops.fused_linear import MurmuraLinear
+from murmura_amd.ops.fused_norm import MurmuraGroupNorm
+from murmura_amd.utils import checkpoint, factories
+
+F = torch.nn.functional
+ACTS = {"none": lambda z: z, "relu": torch.relu, "silu": F.silu, "gelu": F.gelu}
+
+
+def _randn(*shape, seed=0):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed), dtype=torch.float64)
+
+
+@pytest.mark.parametrize("act", ref.ACTIVATIONS)
+def test_definitions_in_64_bits_and_their_gradients(act):
+    x, w, b, r = _randn(3, 6, 4, 5), _randn(6, seed=1), _randn(6, seed=2), _randn(3, 6, 4, 5, seed=3)
+    want = ACTS[act](F.group_norm(x, 3, w, b) + r)
+    # 60 operations in 64 bits on values below 10
+    assert torch.allclose(ops.group_norm_act(x, 3, w, b, act=act, res=r), want, rtol=0, atol=600 * 2.0 ** -53)
+    leaves = [t.requires_grad_(True) for t in (x, w, b, r)]
+    assert torch.autograd.gradcheck(lambda x, w, b, r: ops.group_norm_act(x, 3, w, b, act=act, res=r), leaves)
+    x, w, b, r = _randn(2, 3, 7), _randn(5, 7, seed=1), _randn(5, seed=2), _randn(2, 3, 5, seed=3)
+    want = ACTS[act](F.linear(x, w, b) + r)
+    assert torch.allclose(ops.linear_act(x, w, b, act, r), want, rtol=0, atol=600 * 2.0 ** -53)
+    leaves = [t.requires_grad_(True) for t in (x, w, b, r)]
+    assert torch.autograd.gradcheck(lambda x, w, b, r: ops.linear_act(x, w, b, act, r), leaves)
+
+
+def test_norm_and_linear_refuse():
+    x = torch.randn(2, 6, 3, 3)
+    for bad in (lambda: ops.group_norm_act(x, 4), lambda: ops.group_norm_act(x, 0),
+                lambda: ops.group_norm_act(x[0], 3), lambda: ops.group_norm_act(x, 3, torch.ones(5)),
+                lambda: ops.group_norm_act(x, 3, torch.ones(6), torch.ones(6).double()),
+                lambda: ops.group_norm_act(x, 3, torch.ones(6).bfloat16()),
+                lambda: ops.group_norm_act(x, 3, res=x[:1]), lambda: ops.group_norm_act(x, 3, act="tanh"),
+                lambda: ops.group_norm_act(x, 3, res=x.bfloat16())):
+        with pytest.raises(ValueError):
+            bad()
+    x, w = torch.randn(4, 6), torch.randn(5, 6)
+    for bad in (lambda: ops.linear_act(x, w.t()), lambda: ops.linear_act(x, w[0]),
+                lambda: ops.linear_act(x, w.bfloat16()), lambda: ops.linear_act(x, w, torch.ones(4)),
+                lambda: ops.linear_act(x, w, torch.ones(5).double()), lambda: ops.linear_act(x, w, act="tanh"),
+                lambda: ops.linear_act(x, w, res=torch.ones(5)), lambda: ops.linear_act(x[0, 0], w)):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(ValueError):
+        MurmuraGroupNorm(2, 6, act="swish")
+    with pytest.raises(ValueError):
+        MurmuraLinear(2, 6, act="swish")
+
+
+def test_empty_inputs():
+    for shape in ((0, 4, 3, 3), (2, 4, 0, 3), (0, 4)):
+        assert ops.group_norm_act(torch.zeros(shape), 2, act="silu").shape == shape
+    assert ops.linear_act(torch.zeros(0, 4), torch.zeros(3, 4)).shape == (0, 3)
+    assert torch.equal(ops.linear_act(torch.zeros(2, 0), torch.zeros(3, 0), torch.ones(3)), torch.ones(2, 3))
+
+
+# ------------------------------------------------------------------ AdamW
+def test_adamw_is_torchs_in_32_bits():
+    p = [_randn(7, 5).float(), _randn(11, seed=1).float()]
+    q = [t.clone().requires_grad_(True) for t in p]
+    opt = torch.optim.AdamW(q, lr=1e-2, betas=(0.8, 0.95), eps=1e-6, weight_decay=0.1)
+    state = ops.adamw_state(46, "cpu")
+    for k in range(20):
+        grads = [_randn(*t.shape, seed=10 + k).float() for t in p]
+        for t, g in zip(q, grads):
+            t.grad = g.clone()
+        opt.step()
+        ops.adamw_step(p, grads, *state, 1e-2, betas=(0.8, 0.95), eps=1e-6, weight_decay=0.1)
+    # 20 steps of ten roundings each to 2^-24 of a parameter below 4 or a step below 0.1
+    for a, b in zip(p, q):
+        assert torch.allclose(a, b.detach(), rtol=0, atol=20 * 10 * 2.0 ** -24 * 4)
+    assert int(state[2]) == 20
+
+
+@pytest.mark.parametrize("first", [True, False])
+def test_codes_hold_what_they_decode_to(first):
+    codes = torch.arange(256).repeat(3)[: 2 * 256 + 200].to(torch.uint8)
+    if not first:
+        codes = codes.clamp(max=247)  # the last below the block's scale
+    else:
+        codes = torch.where((codes & 127) > 119, 119, codes.int()).to(torch.uint8)
+    exps = torch.tensor([126, 3, 200], dtype=torch.uint8)
+    values = ref.adamw_decode(codes, exps, first)
+    assert torch.isfinite(values).all()
+    again, e = ref.adamw_encode(values, first, torch.zeros(codes.numel(), dtype=torch.int64))
+    # all were below their scale, so a scale made of the values is that or a smaller one
+    assert torch.equal(ref.adamw_decode(again, e, first), values)
+    assert torch.equal(values.bfloat16().float()[:256], values[:256])
+
+
+def test_codes_round_without_bias_and_keep_what_is_not_finite():
+    n = 1 << 16
+    x = torch.full((n,), 0.3)
+    x[0] = 1.0
+    for first in (True, False):
+        u = ref.adamw_dither(n, 5, 1, "cpu")[0 if first else 1]
+        v = ref.adamw_decode(*ref.adamw_encode(x, first, u), first)
+        # between 0.28125 and 0.3125: a standard deviation of the mean of at most half a step / sqrt(n)
+        assert abs(v[1:].mean() - 0.3) < 5 * 0.03125 / 2 / math.sqrt(n)
+        bad = torch.tensor([math.nan, math.inf, 1.0, 1e-30, 0.0] + [0.5] * 300)
+        c, e = ref.adamw_encode(bad, first, torch.zeros(305, dtype=torch.int64))
+        got = ref.adamw_decode(c, e, first)
+        assert torch.isnan(got[:2]).all() and torch.equal(got[2:3], bad[2:3]) and got[4] == 0
+        assert got[3] == 0 if first else 0 < got[3] <= 2.0 ** -31  # v above zero stays so
+
+
+def test_adamw_refuses_on_the_cpu():
+    p, g = torch.zeros(10), torch.zeros(10)
+    m, v, t = ops.adamw_state(10, "cpu")
+    m8, v8, _ = ops.adamw_state(10, "cpu", 8)
+    for args in (([p], [], m, v, t), ([], [], m, v, t), ([p], [g[:9]], m, v, t), ([p], [g], m[:9], v, t),
+                 ([p], [g], m8, v, t), ([p], [g], m.double(), v.double(), t)):
+        with pytest.raises(RuntimeError):
+            ops.adamw_step(*args, 1e-3)
+    for betas in ((1.0, 0.9), (0.9, -0.1)):
+        with pytest.raises(ValueError):
+            ops.adamw_step(p, g, m, v, t, 1e-3, betas=betas)
+    with pytest.raises(ValueError):
+        ops.adamw_state(10, "cpu", 4)
+    with pytest.raises(ValueError):
+        ops.adamw_dequantize(m8, v8, dtype=torch.float16)
+    assert int(t) == 0
+
+
+def test_adamw_knows_parameters_by_their_memory():
+    w = torch.zeros(4, 3, 3, 2).permute(0, 3, 1, 2)  # channels last
+    g = _randn(4, 2, 3, 3).float()
+    one, two = ops.adamw_state(72, "cpu"), ops.adamw_state(72, "cpu")
+    ops.adamw_step([w], [g], *one, 0.1)
+    flat = torch.zeros(72)
+    ops.adamw_step(flat, g.permute(0, 2, 3, 1).reshape(-1), *two, 0.1)
+    assert torch.equal(w.permute(0, 2, 3, 1).reshape(-1), flat) and torch.equal(one[0], two[0])
+
+
+# -------------------------------------------------- models, nodes, configs
+def _node(model, optimizer=None, shape=(12,), classes=4, dtype=torch.float32, node_id=0):
+    data = TensorDataset(_randn(32, *shape, seed=9).float(), torch.arange(32) % classes)
+    loader = DataLoader(data, batch_size=8)
+    return Node(node_id, model, loader, loader, FedAvgAggregator(), torch.device("cpu"), dtype=dtype,
+                optimizer=optimizer)
+
+
+@pytest.mark.parametrize("cls,kwargs,shape", [
+    (SimpleMLP, dict(in_features=12), (12,)), (WideMLP, dict(in_features=12, hidden=20, num_classes=4), (12,)),
+    (FEMNISTModel, dict(hidden=16, num_classes=4), (1, 28, 28)),
+])
+def test_fused_models_are_their_plain_ones(cls, kwargs, shape):
+    plain, fused = cls(**kwargs), cls(**kwargs, fused=True)
+    assert list(plain.state_dict()) == list(fused.state_dict())
+    fused.load_state_dict(plain.state_dict())
+    x = _randn(5, *shape).float()
+    a, b = plain(x), fused(x)
+    assert torch.allclose(a, b, rtol=0, atol=1e-4 * a.abs().max().item())  # k <= 3136 sums of fp32: 3136 * 2^-24
+    assert any(isinstance(m, MurmuraLinear) for m in fused.modules())
+
+
+def test_resnet_with_group_norm():
+    model = ResNet18(num_classes=4, norm="group", groups=8)
+    norms = [m for m in model.modules() if isinstance(m, MurmuraGroupNorm)]
+    assert len(norms) == 20 and not list(model.buffers())
+    x = _randn(2, 3, 16, 16).float().requires_grad_(True)
+    y = model(x)
+    grads = torch.autograd.grad(y.square().sum(), [x, *model.parameters()])
+    assert y.shape == (2, 4) and all(torch.isfinite(g).all() for g in grads)
+    # a sample's answer does not depend on its batch: convolutions of up to 4608 products in another order
+    assert torch.allclose(model(x[:1]), y[:1], rtol=0, atol=1e-3 * y.abs().max().item())
+    with pytest.raises(ValueError):
+        ResNet18(norm="layer")
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_node_trains_with_adamw(bits, dtype):
+    torch.manual_seed(0)
+    node = _node(SimpleMLP(12, fused=True), AdamWConfig(state_bits=bits), dtype=dtype)
+    before = node.get_state()
+    out = node.local_train(epochs=2, lr=1e-2)
+    assert math.isfinite(out["loss"]) and int(node.optimizer.count) == 8
+    assert (node.get_state() != before).float().mean() > 0.5
+    # the same again gives the same bits
+    torch.manual_seed(0)
+    again = _node(SimpleMLP(12, fused=True), AdamWConfig(state_bits=bits), dtype=dtype)
+    again.local_train(epochs=2, lr=1e-2)
+    assert torch.equal(again.get_state(), node.get_state())
+
+
+def test_node_adamw_leaves_frozen_parameters():
+    model = SimpleMLP(12)
+    model.net[0].weight.requires_grad_(False)
+    node = _node(model, AdamWConfig(weight_decay=0.5))
+    kept = model.net[0].weight.detach().clone()
+    node.local_train(lr=1e-2)
+    assert torch.equal(model.net[0].weight, kept)
+
+
+def test_checkpoint_carries_the_optimizer(tmp_path):
+    torch.manual_seed(0)
+    a = _node(SimpleMLP(12), AdamWConfig(state_bits=8))
+    a.local_train(lr=1e-2)
+    checkpoint.save_checkpoint(tmp_path / "c.pt", 0, [a])
+    blob = checkpoint.load_checkpoint(tmp_path / "c.pt")
+    b = _node(SimpleMLP(12), AdamWConfig(state_bits=8))
+    checkpoint.restore_node_state(b, blob["nodes"][0])
+    a.local_train(lr=1e-2)
+    b.local_train(lr=1e-2)
+    assert torch.equal(a.get_state(), b.get_state()) and int(b.optimizer.count) == 8
+    with pytest.raises(ValueError):
+        checkpoint.restore_node_state(_node(SimpleMLP(12), AdamWConfig(state_bits=32)), blob["nodes"][0])
+    checkpoint.restore_node_state(_node(SimpleMLP(12)), blob["nodes"][0])  # an SGD run takes the parameters
+
+
+def test_configuration_reaches_the_optimizer():
+    config = Config(training={"optimizer": "adamw", "optimizer_bits": 8, "weight_decay": 0.1, "betas": [0.8, 0.9]})
+    got = factories.build_optimizer(config, 3)
+    assert got == AdamWConfig(betas=(0.8, 0.9), weight_decay=0.1, state_bits=8, seed=45)
+    assert factories.build_optimizer(Config(), 0) is None
+    for bad in ({"optimizer": "adam"}, {"optimizer_bits": 4}, {"betas": [0.9, 1.0]}):
+        with pytest.raises(ValueError):
+            Config(training=bad)
+    model = factories.build_model_factory(
+        Config(model={"factory": "models.resnet18", "params": {"norm": "group"}}))()
+    assert isinstance(model.bn1, MurmuraGroupNorm)
