@@ -558,13 +558,14 @@ __global__ __launch_bounds__(NT) void join_kernel(const float* __restrict__ ws, 
   finish<T, ACT>(e, at, at % N, v);
 }
 
-// dz = dy * act'(z) and, for each chunk of rows, its sum over them. 64 columns a block, a wave a
-// row. A relu's z is told by y = relu(z) as well: they are above zero together.
+// dz = dy * act'(z) and, for each chunk of rows, its sum over them (of a single chunk: the bias's
+// gradient). 64 columns a block, a wave a row. A relu's z is told by y = relu(z) as well: they are above zero together.
 template <typename T, int ACT>
 __global__ __launch_bounds__(NT) void act_bwd_kernel(const T* __restrict__ dy,
                                                      const T* __restrict__ z, int64_t M, int64_t N,
                                                      int64_t col_tiles, int64_t chunk,
-                                                     T* __restrict__ dz, float* __restrict__ ws) {
+                                                     T* __restrict__ dz, float* __restrict__ ws,
+                                                     void* __restrict__ db, bool is_float) {
   __shared__ float part[NT / 64][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t c = blockIdx.x % col_tiles * 64 + lane, k = blockIdx.x / col_tiles;
@@ -583,10 +584,13 @@ __global__ __launch_bounds__(NT) void act_bwd_kernel(const T* __restrict__ dy,
   }
   part[wave][lane] = s;
   __syncthreads();
-  if (ws && wave == 0 && c < N) {
+  if ((ws || db) && wave == 0 && c < N) {
 #pragma unroll
     for (int w = 1; w < NT / 64; ++w) s += part[w][lane];
-    ws[k * N + c] = s;
+    if (db)
+      store_param(db, c, is_float, s);
+    else
+      ws[k * N + c] = s;
   }
 }
 
@@ -859,19 +863,22 @@ class LinearAct : public torch::autograd::Function<LinearAct> {
       if (need_b) db.zero_();
     } else if (need_b || act != ACT_NONE) {
       const int64_t cols = ceil_div(N, 64);
-      const int64_t chunk = std::max<int64_t>(16, ceil_div(M, std::max<int64_t>(1, 2048 / cols)));
+      // up to 128 rows one chunk, which needs no second launch; else as many as fill the CUs
+      const int64_t chunk = M <= 128 ? M : std::max<int64_t>(16, ceil_div(M, std::max<int64_t>(1, 2048 / cols)));
       const int64_t chunks = ceil_div(M, chunk);
       TORCH_CHECK(cols * chunks < (1LL << 31), "linear_act: too many blocks");
       Tensor ws;
-      if (need_b) ws = at::empty({chunks * N}, dy.options().dtype(at::kFloat));
-      float* wp = need_b ? ws.data_ptr<float>() : nullptr;
+      const bool bias_float = need_b && db.scalar_type() == at::kFloat;
+      if (need_b && chunks > 1) ws = at::empty({chunks * N}, dy.options().dtype(at::kFloat));
+      float* wp = ws.defined() ? ws.data_ptr<float>() : nullptr;
+      void* once = need_b && chunks == 1 ? db.data_ptr() : nullptr;
       MM_DISPATCH_TYPE(dy, MM_DISPATCH_ACT(act, {
         act_bwd_kernel<T, ACT><<<(unsigned)(cols * chunks), NT, 0, st>>>(
-            (const T*)ptr(dy), (const T*)ptr(saved[2]), M, N, cols, chunk, (T*)dz.data_ptr(), wp);
+            (const T*)ptr(dy), (const T*)ptr(saved[2]), M, N, cols, chunk, (T*)dz.data_ptr(), wp,
+            once, bias_float);
       }));
-      if (need_b)
-        bias_grad_kernel<<<(unsigned)cols, NT, 0, st>>>(wp, chunks, N, db.scalar_type() == at::kFloat,
-                                                       db.data_ptr());
+      if (wp)
+        bias_grad_kernel<<<(unsigned)cols, NT, 0, st>>>(wp, chunks, N, bias_float, db.data_ptr());
       check_launch("linear_act backward");
     }
     const Tensor dzm = dz.view({M, N});
