@@ -24,6 +24,7 @@ struct Operand {
   const void* p;
   int64_t ld;  // values from one row in memory to the next
   bool whole;  // rows and base allow 16-byte loads
+  bool words;  // or 4-byte ones
 };
 
 struct Epilogue {
@@ -275,10 +276,12 @@ typedef __attribute__((address_space(3))) s4 lds_s4;
 constexpr int ROW_BYTES = 128;
 
 // ROWS rows of an operand: HR of each STRIDE, from the first on
-template <typename T, bool ACROSS, int ROWS, int THREADS, int HR, int STRIDE>
+// (LB bytes a lane and load: 16 where rows and their ends lie on 16 bytes, else 4)
+template <typename T, bool ACROSS, int ROWS, int THREADS, int HR, int STRIDE, int LB>
 struct Direct {
   static constexpr int E = 16 / sizeof(T), FK = ROW_BYTES / sizeof(T);  // values of a chunk, of a row
-  static constexpr int LOADS = ROWS * (FK / E) / THREADS;
+  static constexpr int U = LB / sizeof(T), PARTS = E / U;  // values of a load, loads of a chunk
+  static constexpr int LOADS = ROWS * (FK / U) / THREADS;
   static constexpr int SIZE = ROWS * FK;
   static constexpr int CH = ROWS / E;        // chunks of a row of k
   static constexpr int PAIRS = ROWS / 16;    // 16 columns of it
@@ -291,20 +294,20 @@ struct Direct {
     return sizeof(T) == 4 ? (k >> 2) & LOW : (k & LOW) | ((k >> 3) & HIGH) << 2;
   }
   __device__ __forceinline__ static void slot(int i, int& r, int& k) {
-    const int s = i * THREADS + threadIdx.x;
+    const int s = (i * THREADS + threadIdx.x) / PARTS, part = threadIdx.x % PARTS * U;
     if (ACROSS) {
       k = s / CH;
-      r = ((s % CH) ^ g_of(k) * (16 / E)) * E;
+      r = ((s % CH) ^ g_of(k) * (16 / E)) * E + part;
     } else {
       r = s / 8;
-      k = ((s % 8) ^ (r >> 1 & 7)) * E;
+      k = ((s % 8) ^ (r >> 1 & 7)) * E + part;
     }
   }
   __device__ __forceinline__ void init(const Operand& o, int64_t r0, int64_t k0, int64_t R) {
     step = ACROSS ? FK * o.ld : FK;
-    r0 = min(r0, R - (ACROSS ? E : 1));  // rows that start behind the end
+    r0 = min(r0, R - (ACROSS ? U : 1));  // rows that start behind the end
     base = (const T*)o.p + (ACROSS ? k0 * o.ld + r0 : r0 * o.ld + k0);
-    const int last = (int)min(R - r0, (int64_t)(ROWS / HR * STRIDE)) - (ACROSS ? E : 1);
+    const int last = (int)min(R - r0, (int64_t)(ROWS / HR * STRIDE)) - (ACROSS ? U : 1);
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       int r, k;
@@ -317,11 +320,17 @@ struct Direct {
   __device__ __forceinline__ void load(T* lds, int wave) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const unsigned to = (unsigned)(uintptr_t)(lds_void*)(lds + (i * THREADS + wave * 64) * E);
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                   :
-                   : "s"(to), "v"(at[i]), "s"(base)
-                   : "memory");
+      const unsigned to = (unsigned)(uintptr_t)(lds_void*)(lds + (i * THREADS + wave * 64) * U);
+      if constexpr (LB == 16)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                     :
+                     : "s"(to), "v"(at[i]), "s"(base)
+                     : "memory");
+      else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
+                     :
+                     : "s"(to), "v"(at[i]), "s"(base)
+                     : "memory");
     }
     base += step;
   }
@@ -333,15 +342,15 @@ struct Direct {
       int r, k;
       slot(i, r, k);
       const T* from = p + at[i] / sizeof(T);
-      Vec<T, E> v = {};
-      if ((ACROSS ? k + 1 : k + E) <= left) {
-        v = *(const Vec<T, E>*)from;
+      Vec<T, U> v = {};
+      if ((ACROSS ? k + 1 : k + U) <= left) {
+        v = *(const Vec<T, U>*)from;
       } else if (!ACROSS) {
 #pragma unroll
-        for (int j = 0; j < E; ++j)
+        for (int j = 0; j < U; ++j)
           if (k + j < left) v.e[j] = from[j];
       }
-      *(Vec<T, E>*)(lds + (i * THREADS + threadIdx.x) * E) = v;
+      *(Vec<T, U>*)(lds + (i * THREADS + threadIdx.x) * U) = v;
     }
   }
   // 16 rows from `row`, half ks of the step's k: lane l has row l % 16, chunk l / 16 of the half
@@ -391,13 +400,13 @@ __device__ __forceinline__ void tile_of(int64_t b, int64_t rows, int64_t cols, i
   c = t % band / height;
 }
 
-template <typename T, bool AX, bool BX, int ACT, int BM, int BN, int WM, int WN>
+template <typename T, bool AX, bool BX, int ACT, int BM, int BN, int WM, int WN, int LB>
 __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_large_kernel(
     Operand a, Operand b, int64_t M, int64_t N, int64_t Kd, int64_t a_end, int64_t b_end, int64_t k_part,
     int64_t row_tiles, int64_t col_tiles, Epilogue e, float* __restrict__ ws) {
   constexpr int THREADS = 64 * WM * WN, FM = BM / WM / 16, FN = BN / WN / 16, H = FM / 2;
-  using A = Direct<T, AX, BM / 2, THREADS, H * 16, FM * 16>;  // the upper rows, or the lower ones
-  using B = Direct<T, BX, BN, THREADS, BN, BN>;
+  using A = Direct<T, AX, BM / 2, THREADS, H * 16, FM * 16, LB>;  // the upper rows, or the lower ones
+  using B = Direct<T, BX, BN, THREADS, BN, BN, LB>;
   constexpr int FK = A::FK;
   __shared__ __attribute__((aligned(1024))) T lds[2 * (2 * A::SIZE + B::SIZE)];
   // per buffer: upper rows, lower rows, B
@@ -456,6 +465,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_large_kernel(
   // A step's loads but the oldest of them may still be on their way at a barrier; at the sum's end,
   // where nothing new is loaded, all are waited for.
   constexpr int AHEAD = 2 * A::LOADS + B::LOADS;
+  static_assert(AHEAD < 64, "the count of outstanding loads has 6 bits");
   const auto barrier = [&](bool all) {
     if (all)
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -616,7 +626,8 @@ const void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; 
 
 Operand operand(const Tensor& t) {
   const int64_t size = t.element_size(), ld = t.size(0) > 1 ? t.stride(0) : 0;
-  return {t.data_ptr(), ld, ld * size % 16 == 0 && (uintptr_t)t.data_ptr() % 16 == 0};
+  const uintptr_t at = (uintptr_t)t.data_ptr();
+  return {t.data_ptr(), ld, ld * size % 16 == 0 && at % 16 == 0, ld * size % 4 == 0 && at % 4 == 0};
 }
 
 bool rows_of_8(int64_t N, std::initializer_list<const void*> ptrs) {
@@ -670,12 +681,12 @@ constexpr TileShape TILES[] = {
 // on. bf16, M x K x N: 2048x12288x4096 takes 278 us in tiles of 256x256 and 205 in two parts, 184 in
 // 256x128, 198 in 128x128; 1024x1024x1024 14 in 128x128, 9 in 64x64; 64x3136x2048 19 in 64x64 whole,
 // 8.5 in 8 parts; 1x4096x12288 39 whole, 19 in 2 parts, 22 in 8.
-Choice choose(int64_t M, int64_t N, int64_t Kd, int64_t elem) {
+Choice choose(int64_t M, int64_t N, int64_t Kd, int64_t elem, bool by_words) {
   Choice best{0, 1};
   double least = 1e30;
   const int64_t steps = ceil_div(Kd * elem, ROW_BYTES);
   const double bytes = (double)(M * Kd + N * Kd + M * N) * elem;
-  for (int t = 0; t < 4; ++t) {
+  for (int t = by_words ? 2 : 0; t < 4; ++t) {
     const TileShape& s = TILES[t];
     const int64_t tiles = ceil_div(M, s.bm) * ceil_div(N, s.bn);
     for (int64_t parts = 1; parts <= 64 && (parts == 1 || (steps >= 2 * parts && tiles * parts <= 1536));
@@ -695,13 +706,13 @@ Choice choose(int64_t M, int64_t N, int64_t Kd, int64_t elem) {
   return best;
 }
 
-template <typename T, bool AX, bool BX, int ACT, int BM, int BN, int WM, int WN>
+template <typename T, bool AX, bool BX, int ACT, int BM, int BN, int WM, int WN, int LB = 16>
 void launch_large(const Operand& a, const Operand& b, int64_t M, int64_t N, int64_t Kd, int64_t Ma,
                   int64_t Nb, int64_t parts, const Epilogue& e, float* ws, hipStream_t st) {
   const int64_t rows = ceil_div(M, BM), cols = ceil_div(N, BN), values = ROW_BYTES / sizeof(T);
   TORCH_CHECK(rows * cols < (1LL << 31), "linear_act: too many tiles");
   const int64_t part = ceil_div(ceil_div(Kd, parts), values) * values;
-  gemm_large_kernel<T, AX, BX, ACT, BM, BN, WM, WN>
+  gemm_large_kernel<T, AX, BX, ACT, BM, BN, WM, WN, LB>
       <<<dim3((unsigned)(rows * cols), (unsigned)parts), 64 * WM * WN, 0, st>>>(a, b, M, N, Kd, Ma, Nb, part,
                                                                               rows, cols, e, ws);
 }
@@ -716,10 +727,14 @@ void launch_small(const Operand& a, const Operand& b, int64_t M, int64_t N, int6
       a, b, M, N, Kd, part, cols, e, ws);
 }
 
-// A product of rows off the 16 bytes is worth a copy of them from this many multiplications on:
-// 509x561x250 in bf16 takes 13 us as it lies and 21 with the copy, 2000x561x250 20 and 22,
-// 1000x1001x999 43 and 27, 4001x4003x4099 2435 and 198.
-constexpr double PAD_FROM = 8e8;
+// Rows off the 16 bytes. Where they lie on 4, as fp32 always does, lanes load 4 bytes each: fp32
+// 509x561x250 takes 15 us so and 14 through registers, 2000x999x1003 48 and 92, copied 52;
+// 4001x4003x4099 1033, 2600 and 1074. bf16 needs more loads a product and is copied from PAD_WORDS
+// multiplications on: 2002^3 takes 49 us by words and 46 copied, 3002^3 130 and 107, 4002^3 205 and
+// 152. Rows of bf16 off the 4 bytes go through registers, and are copied from PAD_ODD on: 509x561x250
+// takes 13 us so and 21 copied, 2000x561x250 20 and 22, 1000x1001x999 43 and 17, 4001x4003x4099 2435
+// and 198.
+constexpr double PAD_WORDS = 8e9, PAD_ODD = 8e8;
 
 // out [M, N] = A B^T over Kd, A and B with k along (or across) their rows in memory
 template <bool AX, bool BX>
@@ -732,11 +747,15 @@ void gemm(const Tensor& a, const Tensor& b, int64_t M, int64_t N, int64_t Kd, co
   // offsets within a tile are 32 bits
   bool large = Kd > 0 && std::max(oa.ld, ob.ld) * 256 * elem < (1LL << 32);
   const bool fits_a = oa.whole && (!AX || M % E == 0), fits_b = ob.whole && (!BX || N % E == 0);
+  const bool words = oa.words && ob.words && (!AX || M * elem % 4 == 0) && (!BX || N * elem % 4 == 0);
   int64_t Ma = M, Nb = N;  // rows that may be read
+  bool by_words = false;
   Tensor padded;
   if (large && !(fits_a && fits_b)) {
-    large = (double)M * N * Kd >= PAD_FROM;
-    if (large) {
+    const double work = (double)M * N * Kd;
+    by_words = words && (elem == 4 || work < PAD_WORDS);
+    large = by_words || work >= PAD_ODD;
+    if (large && !by_words) {
       // k is filled up to whole steps with zeros, the rows that a product goes over to whole vectors
       const int64_t step = ROW_BYTES / elem;
       const auto pad = [&](const Tensor& t, const Operand& o, bool fits, bool across) {
@@ -750,14 +769,14 @@ void gemm(const Tensor& a, const Tensor& b, int64_t M, int64_t N, int64_t Kd, co
       pa.to = padded.data_ptr();
       pb.to = (char*)pa.to + pa.rows * pa.ld * elem;
       MM_DISPATCH_TYPE(like, (pad_kernel<T><<<(unsigned)(pa.rows + pb.rows), NT, 0, st>>>(pa, pb)));
-      if (!fits_a) oa = {pa.to, pa.ld, true}, Ma = AX ? pa.ld : M;
-      if (!fits_b) ob = {pb.to, pb.ld, true}, Nb = BX ? pb.ld : N;
+      if (!fits_a) oa = {pa.to, pa.ld, true, true}, Ma = AX ? pa.ld : M;
+      if (!fits_b) ob = {pb.to, pb.ld, true, true}, Nb = BX ? pb.ld : N;
       if (!fits_a && !fits_b) Kd = ceil_div(Kd, step) * step;
     }
   }
   Choice c{0, 1};
   if (large) {
-    c = choose(M, N, Kd, elem);
+    c = choose(M, N, Kd, elem, by_words);
   } else {
     // few tiles: the sum is split over k, 128 values a part at least
     c.parts = std::max<int64_t>(1, std::min(ceil_div(512, ceil_div(M, 64) * ceil_div(N, 64)), Kd / 128));
@@ -770,6 +789,10 @@ void gemm(const Tensor& a, const Tensor& b, int64_t M, int64_t N, int64_t Kd, co
       if constexpr (ACT == ACT_NONE || !(AX || BX)) {  // only the forward product has an epilogue
         if (!large)
           launch_small<T, AX, BX, ACT>(oa, ob, M, N, Kd, c.parts, e, wp, st);
+        else if (by_words && c.tile == 2)
+          launch_large<T, AX, BX, ACT, 128, 128, 2, 2, 4>(oa, ob, M, N, Kd, Ma, Nb, c.parts, e, wp, st);
+        else if (by_words)
+          launch_large<T, AX, BX, ACT, 64, 64, 2, 2, 4>(oa, ob, M, N, Kd, Ma, Nb, c.parts, e, wp, st);
         else if (c.tile == 0)
           launch_large<T, AX, BX, ACT, 256, 256, 2, 4>(oa, ob, M, N, Kd, Ma, Nb, c.parts, e, wp, st);
         else if (c.tile == 1)

@@ -244,7 +244,7 @@ def _linear_check(x, w, b, act, res, dy):
 
 
 LINEAR_SHAPES = [
-    (600, 1500, 1000), (1023, 1031, 1029), (1300, 700, 1100), (8, 8200, 520), (1500, 64, 1600),
+    (600, 1500, 1000), (34, 42, 66), (258, 262, 514), (2050, 2002, 1950), (1023, 1031, 1029), (1300, 700, 1100), (8, 8200, 520), (1500, 64, 1600),
     (1, 1, 1), (1, 64, 128), (1, 561, 250), (3, 33, 65), (7, 8, 16), (16, 512, 96), (17, 100, 10), (64, 3136, 64),
     (64, 128, 62), (65, 129, 127), (130, 64, 257), (300, 72, 200), (257, 512, 264), (2, 4000, 130), (520, 40, 512),
     (512, 192, 520),
