@@ -37,10 +37,11 @@ struct Epilogue {
   bool whole;  // 8 columns of a row lie on 16 bytes, in all of these
 };
 
+// What a store may overwrite is not loaded ahead of it: a caller with several values loads bias and
+// residual for all of them first.
 template <typename T, int ACT>
-__device__ __forceinline__ void finish(const Epilogue& e, int64_t at, int64_t col, float v) {
-  float z = v + load_param(e.bias, col, e.bias_float, 0.f);
-  if (e.res) z += to_float(((const T*)e.res)[at]);
+__device__ __forceinline__ void finish(const Epilogue& e, int64_t at, float v, float bias, float res) {
+  const float z = v + bias + res;
   if (e.z) ((T*)e.z)[at] = from_float<T>(z);
   ((T*)e.out)[at] = from_float<T>(act_fwd<ACT>(z));
 }
@@ -63,15 +64,14 @@ struct Eight {  // 8 values that lie on 16 bytes
 // 8 columns of a row, which lie on 16 bytes
 template <typename T, int ACT>
 __device__ __forceinline__ void finish8(const Epilogue& e, int64_t at, const float (&bias)[8],
-                                        const float* v) {
+                                        Eight<T>& res, const float* v) {
   float z[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) z[i] = v[i] + bias[i];
   Eight<T> o;
   if (e.res) {
-    o.load(e.res, at);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) z[i] += to_float(o[i]);
+    for (int i = 0; i < 8; ++i) z[i] += to_float(res[i]);
   }
   if (e.z) {
 #pragma unroll
@@ -229,7 +229,8 @@ __global__ __launch_bounds__(NT) void gemm_kernel(Operand a, Operand b, int64_t 
         if (ws)
           ws[(blockIdx.y * M + r) * N + c] = acc[i][j][q];
         else
-          finish<T, ACT>(e, r * N + c, c, acc[i][j][q]);
+          finish<T, ACT>(e, r * N + c, acc[i][j][q], load_param(e.bias, c, e.bias_float, 0.f),
+                         e.res ? to_float(((const T*)e.res)[r * N + c]) : 0.f);
       }
 }
 
@@ -543,14 +544,33 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_large_kernel(
     const float* row = mine + lane / LANES * PITCH + lane % LANES * 8;
     const int64_t r = m0 + wm + i * 16 + lane / LANES;
     if (inside) {
+      Eight<T> res[32 / DOWN];
+      if (e.res) {
 #pragma unroll
-      for (int k = 0; k < 32; k += DOWN) finish8<T, ACT>(e, (r + k) * N + c, bias, row + k * PITCH);
-    } else {  // a row at a time, a value a lane
-      const int64_t one = n0 + wn + lane % COLS;
-#pragma unroll 4
-      for (int k = lane / COLS; k < 32; k += 64 / COLS) {
-        const int64_t down = m0 + wm + i * 16 + k;
-        if (down < M && one < N) finish<T, ACT>(e, down * N + one, one, mine[k * PITCH + lane % COLS]);
+        for (int k = 0; k < 32 / DOWN; ++k) res[k].load(e.res, (r + k * DOWN) * N + c);
+      }
+#pragma unroll
+      for (int k = 0; k < 32 / DOWN; ++k)
+        finish8<T, ACT>(e, (r + k * DOWN) * N + c, bias, res[k], row + k * DOWN * PITCH);
+    } else {  // a row at a time, a value a lane, the residuals of eight rows ahead
+      constexpr int NEXT = 64 / COLS;
+      const int64_t one = n0 + wn + lane % COLS, top = m0 + wm + i * 16 + lane / COLS;
+      const float shift = one < N ? load_param(e.bias, one, e.bias_float, 0.f) : 0.f;
+#pragma unroll 1
+      for (int k = 0; k < 32; k += 8 * NEXT) {
+        float res[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const int64_t down = top + k + q * NEXT;
+          res[q] = e.res && down < M && one < N ? to_float(((const T*)e.res)[down * N + one]) : 0.f;
+        }
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const int64_t down = top + k + q * NEXT;
+          if (down < M && one < N)
+            finish<T, ACT>(e, down * N + one,
+                           mine[(k + q * NEXT + lane / COLS) * PITCH + lane % COLS], shift, res[q]);
+        }
       }
     }
     __builtin_amdgcn_wave_barrier();
@@ -565,7 +585,8 @@ __global__ __launch_bounds__(NT) void join_kernel(const float* __restrict__ ws, 
   if (at >= total) return;
   float v = 0.f;
   for (int s = 0; s < parts; ++s) v += ws[s * total + at];
-  finish<T, ACT>(e, at, at % N, v);
+  finish<T, ACT>(e, at, v, load_param(e.bias, at % N, e.bias_float, 0.f),
+                 e.res ? to_float(((const T*)e.res)[at]) : 0.f);
 }
 
 // dz = dy * act'(z) and, for each chunk of rows, its sum over them (of a single chunk: the bias's
@@ -604,19 +625,19 @@ __global__ __launch_bounds__(NT) void act_bwd_kernel(const T* __restrict__ dy,
   }
 }
 
-__global__ __launch_bounds__(NT) void bias_grad_kernel(const float* __restrict__ ws, int64_t chunks,
-                                                       int64_t N, bool is_float, void* db) {
-  __shared__ float part[NT / 64][64];
+__global__ __launch_bounds__(1024) void bias_grad_kernel(const float* __restrict__ ws, int64_t chunks,
+                                                         int64_t N, bool is_float, void* db) {
+  __shared__ float part[16][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t c = (int64_t)blockIdx.x * 64 + lane;
   float s = 0.f;
   if (c < N)
-    for (int64_t k = wave; k < chunks; k += NT / 64) s += ws[k * N + c];
+    for (int64_t k = wave; k < chunks; k += 16) s += ws[k * N + c];
   part[wave][lane] = s;
   __syncthreads();
   if (wave == 0 && c < N) {
 #pragma unroll
-    for (int w = 1; w < NT / 64; ++w) s += part[w][lane];
+    for (int w = 1; w < 16; ++w) s += part[w][lane];
     store_param(db, c, is_float, s);
   }
 }
@@ -694,7 +715,8 @@ Choice choose(int64_t M, int64_t N, int64_t Kd, int64_t elem, bool by_words) {
       const int64_t a_cu = ceil_div(tiles * parts, 256), full = a_cu / s.per_cu, rest = a_cu % s.per_cu;
       const double* us = elem == 2 ? s.bf16_us : s.fp32_us;
       const double part = (double)ceil_div(steps, parts);
-      double cost = full * (part * us[s.per_cu - 1] + 2) + (rest ? part * us[rest - 1] + 2 : 0);
+      const double last = 2 + 1.5e-4 * s.bm * s.bn * s.per_cu;  // and the tile's way out
+      double cost = full * (part * us[s.per_cu - 1] + last) + (rest ? part * us[rest - 1] + last : 0);
       cost = std::max(cost, bytes / 5e6 * std::max(1.0, 256.0 / (tiles * parts)));
       if (parts > 1) cost += 6 + (double)M * N * 8 * parts / 5e6;
       if (cost < least) {
@@ -886,8 +908,10 @@ class LinearAct : public torch::autograd::Function<LinearAct> {
       if (need_b) db.zero_();
     } else if (need_b || act != ACT_NONE) {
       const int64_t cols = ceil_div(N, 64);
-      // up to 128 rows one chunk, which needs no second launch; else as many as fill the CUs
-      const int64_t chunk = M <= 128 ? M : std::max<int64_t>(16, ceil_div(M, std::max<int64_t>(1, 2048 / cols)));
+      // up to 128 rows one chunk, which needs no second launch; else as many as fill the CUs, and
+      // 256 at most, which 16 waves join in 16 steps
+      const int64_t most = std::min<int64_t>(256, std::max<int64_t>(1, 2048 / cols));
+      const int64_t chunk = M <= 128 ? M : std::max<int64_t>(16, ceil_div(M, most));
       const int64_t chunks = ceil_div(M, chunk);
       TORCH_CHECK(cols * chunks < (1LL << 31), "linear_act: too many blocks");
       Tensor ws;
@@ -901,7 +925,7 @@ class LinearAct : public torch::autograd::Function<LinearAct> {
             once, bias_float);
       }));
       if (wp)
-        bias_grad_kernel<<<(unsigned)cols, NT, 0, st>>>(wp, chunks, N, bias_float, db.data_ptr());
+        bias_grad_kernel<<<(unsigned)cols, 1024, 0, st>>>(wp, chunks, N, bias_float, db.data_ptr());
       check_launch("linear_act backward");
     }
     const Tensor dzm = dz.view({M, N});
