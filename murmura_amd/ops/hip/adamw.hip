@@ -540,12 +540,11 @@ std::tuple<Tensor, Tensor> adamw_decode(const std::vector<Tensor>& exp_avg,
   Tensor m = at::empty({P}, options), v = at::empty({P}, options);
   if (P == 0) return {m, v};
   const int64_t blocks = ceil_div(P, (int64_t)NT * 8);
-  TORCH_CHECK(blocks < (1LL << 31), "adamw_dequantize: too many values");
   Moments mo{exp_avg[0].data_ptr(), exp_avg_sq[0].data_ptr(), (unsigned char*)exp_avg[1].data_ptr(),
              (unsigned char*)exp_avg_sq[1].data_ptr(), false};
   mo.whole = ((uintptr_t)mo.m | (uintptr_t)mo.v) % 8 == 0;
   MM_DISPATCH_TYPE(m, {
-    adamw_decode_kernel<T><<<dim3((unsigned)blocks, 2), NT, 0, stream_of(m)>>>(
+    adamw_decode_kernel<T><<<dim3(grid_of(blocks, NT, "adamw_dequantize"), 2), NT, 0, stream_of(m)>>>(
         mo, P, (T*)m.data_ptr(), (T*)v.data_ptr());
   });
   check_launch("adamw_dequantize");

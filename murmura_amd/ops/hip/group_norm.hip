@@ -132,34 +132,35 @@ __device__ __forceinline__ float block_sum(float v, float* lds) {
   return s;
 }
 
-// one block a group: joins the chunks' statistics
+// joins the chunks' statistics, a block a group
 __global__ __launch_bounds__(NT) void gn_join_stats_kernel(const float2* __restrict__ ws, Shape s,
-                                                           float eps, float* __restrict__ mean,
+                                                           int64_t all, float eps,
+                                                           float* __restrict__ mean,
                                                            float* __restrict__ rstd) {
   __shared__ float lds[NW];
-  const int64_t n = blockIdx.x / s.G;
-  const int g = blockIdx.x % s.G;
   const int64_t chunk_rows = (int64_t)(NT >> s.lanes) * K;
-  const float2* w = ws + n * s.S * s.C + g * s.Cg;
   const int64_t entries = (int64_t)s.S * s.Cg;
-  float sum = 0.f;
-  for (int64_t e = threadIdx.x; e < entries; e += NT) {
-    const int64_t k = e / s.Cg;
-    sum += w[k * s.C + e % s.Cg].x * (float)min(chunk_rows, s.R - k * chunk_rows);
-  }
-  const float inv = 1.f / ((float)s.R * (float)s.Cg);
-  const float mu = block_sum(sum, lds) * inv;
-  float m2 = 0.f;
-  for (int64_t e = threadIdx.x; e < entries; e += NT) {
-    const int64_t k = e / s.Cg;
-    const float2 q = w[k * s.C + e % s.Cg];
-    const float d = q.x - mu;
-    m2 += q.y + d * d * (float)min(chunk_rows, s.R - k * chunk_rows);
-  }
-  m2 = block_sum(m2, lds);
-  if (threadIdx.x == 0) {
-    mean[blockIdx.x] = mu;
-    rstd[blockIdx.x] = 1.f / sqrtf(m2 * inv + eps);
+  for (int64_t b = blockIdx.x; b < all; b += gridDim.x) {
+    const float2* w = ws + b / s.G * s.S * s.C + b % s.G * s.Cg;
+    float sum = 0.f;
+    for (int64_t e = threadIdx.x; e < entries; e += NT) {
+      const int64_t k = e / s.Cg;
+      sum += w[k * s.C + e % s.Cg].x * (float)min(chunk_rows, s.R - k * chunk_rows);
+    }
+    const float inv = 1.f / ((float)s.R * (float)s.Cg);
+    const float mu = block_sum(sum, lds) * inv;
+    float m2 = 0.f;
+    for (int64_t e = threadIdx.x; e < entries; e += NT) {
+      const int64_t k = e / s.Cg;
+      const float2 q = w[k * s.C + e % s.Cg];
+      const float d = q.x - mu;
+      m2 += q.y + d * d * (float)min(chunk_rows, s.R - k * chunk_rows);
+    }
+    m2 = block_sum(m2, lds);
+    if (threadIdx.x == 0) {
+      mean[b] = mu;
+      rstd[b] = 1.f / sqrtf(m2 * inv + eps);
+    }
   }
 }
 
@@ -255,28 +256,30 @@ __global__ __launch_bounds__(NT) void gn_bwd_sums_kernel(
   }
 }
 
-// one block a group: avg(dz*gamma), avg(dz*gamma*xhat)
+// avg(dz*gamma), avg(dz*gamma*xhat), a block a group
 __global__ __launch_bounds__(NT) void gn_join_sums_kernel(const float2* __restrict__ ws, Shape s,
+                                                          int64_t all,
                                                           const void* __restrict__ gamma, bool wf,
                                                           float2* __restrict__ avg) {
   __shared__ float lds[NW];
-  const int64_t n = blockIdx.x / s.G;
-  const int g = blockIdx.x % s.G;
-  const float2* w = ws + n * s.S * s.C + g * s.Cg;
   const int64_t entries = (int64_t)s.S * s.Cg;
-  float sz = 0.f, sx = 0.f;
-  for (int64_t e = threadIdx.x; e < entries; e += NT) {
-    const int64_t k = e / s.Cg;
-    const int c = (int)(e % s.Cg);
-    const float2 q = w[k * s.C + c];
-    const float ga = load_param(gamma, g * s.Cg + c, wf, 1.f);
-    sz += q.x * ga;
-    sx += q.y * ga;
+  for (int64_t b = blockIdx.x; b < all; b += gridDim.x) {
+    const int g = (int)(b % s.G);
+    const float2* w = ws + b / s.G * s.S * s.C + g * s.Cg;
+    float sz = 0.f, sx = 0.f;
+    for (int64_t e = threadIdx.x; e < entries; e += NT) {
+      const int64_t k = e / s.Cg;
+      const int c = (int)(e % s.Cg);
+      const float2 q = w[k * s.C + c];
+      const float ga = load_param(gamma, g * s.Cg + c, wf, 1.f);
+      sz += q.x * ga;
+      sx += q.y * ga;
+    }
+    const float inv = 1.f / ((float)s.R * (float)s.Cg);
+    sz = block_sum(sz, lds) * inv;
+    sx = block_sum(sx, lds) * inv;
+    if (threadIdx.x == 0) avg[b] = make_float2(sz, sx);
   }
-  const float inv = 1.f / ((float)s.R * (float)s.Cg);
-  sz = block_sum(sz, lds) * inv;
-  sx = block_sum(sx, lds) * inv;
-  if (threadIdx.x == 0) avg[blockIdx.x] = make_float2(sz, sx);
 }
 
 template <typename T, int V, int ACT>
@@ -830,8 +833,7 @@ Shape shape_of(const Image& im, int64_t groups, int V) {
   while (s.lanes < 6 && (1 << s.lanes) * V < s.C) ++s.lanes;
   s.tiles = (int)ceil_div(s.C, (int64_t)(1 << s.lanes) * V);
   const int64_t S = ceil_div(s.R, (int64_t)(NT >> s.lanes) * K);
-  TORCH_CHECK(im.N * s.tiles * S < (1LL << 31) && im.N * groups < (1LL << 31),
-              "group_norm_act: too many blocks");
+  grid_of(im.N * s.tiles * S, NT, "group_norm_act");
   s.S = (int)S;
   return s;
 }
@@ -860,7 +862,7 @@ Plan plan_of(const Image& im, int64_t groups, int V, int64_t elem, int max_threa
     int lanes = 0;
     while ((1 << lanes) * V < c) ++lanes;
     const int64_t blocks = im.N * (G / k);
-    if (blocks >= (1LL << 31)) continue;
+    if (blocks * max_threads >= (1LL << 32)) continue;
     // four rows a thread keep enough loads on their way; `most` are what registers hold
     int threads = 64;
     while (threads < max_threads && (threads >> lanes) * 4 < im.R) threads *= 2;
@@ -942,8 +944,8 @@ void normalise(Forward& f, int64_t groups, double eps, int64_t act) {
   const unsigned blocks = (unsigned)(im.N * s.tiles * s.S);
   MM_DISPATCH_TYPE(x, GN_DISPATCH_VEC(vec, {
     gn_stats_kernel<T, V><<<blocks, NT, 0, st>>>((const T*)ptr(x), s, (float2*)ws.data_ptr());
-    gn_join_stats_kernel<<<(unsigned)(im.N * groups), NT, 0, st>>>(
-        (const float2*)ws.data_ptr(), s, (float)eps, mean.data_ptr<float>(), rstd.data_ptr<float>());
+    gn_join_stats_kernel<<<(unsigned)std::min<int64_t>(im.N * groups, 1 << 20), NT, 0, st>>>(
+        (const float2*)ws.data_ptr(), s, im.N * groups, (float)eps, mean.data_ptr<float>(), rstd.data_ptr<float>());
     MM_DISPATCH_ACT(act, (gn_apply_kernel<T, V, ACT><<<blocks, NT, 0, st>>>(
         (const T*)ptr(x), (const T*)ptr(res), s, mean.data_ptr<float>(), rstd.data_ptr<float>(),
         ptr(w), ptr(b), wf, (T*)y.data_ptr())));
@@ -995,8 +997,8 @@ Grads backward_of(const Tensor& dy, const Tensor& x, int64_t groups, const Tenso
         (const T*)ptr(x), (const T*)ptr(dy), (const T*)ptr(res), s, mean.data_ptr<float>(),
         rstd.data_ptr<float>(), ptr(w), ptr(b), wf, (T*)ptr(g.dres), (float2*)ws.data_ptr())));
     if (need_dx) {
-      gn_join_sums_kernel<<<(unsigned)(im.N * groups), NT, 0, st>>>(
-          (const float2*)ws.data_ptr(), s, ptr(w), wf, (float2*)avg.data_ptr());
+      gn_join_sums_kernel<<<(unsigned)std::min<int64_t>(im.N * groups, 1 << 20), NT, 0, st>>>(
+          (const float2*)ws.data_ptr(), s, im.N * groups, ptr(w), wf, (float2*)avg.data_ptr());
       MM_DISPATCH_ACT(act, (gn_bwd_dx_kernel<T, V, ACT><<<blocks, NT, 0, st>>>(
           (const T*)ptr(x), (const T*)ptr(dy), (const T*)ptr(res), s, mean.data_ptr<float>(),
           rstd.data_ptr<float>(), (const float2*)avg.data_ptr(), ptr(w), ptr(b), wf,

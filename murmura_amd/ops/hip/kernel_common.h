@@ -185,6 +185,12 @@ inline unsigned int magic_of(int64_t d) {
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// a grid of so many blocks: its threads are counted in 32 bits
+inline unsigned grid_of(int64_t blocks, int64_t threads, const char* what) {
+  TORCH_CHECK(blocks > 0 && blocks * threads < (1LL << 32), what, ": too many values for one launch");
+  return (unsigned)blocks;
+}
+
 inline void check_launch(const char* what) {
   const hipError_t e = hipGetLastError();
   TORCH_CHECK(e == hipSuccess, what, ": launch failed: ", hipGetErrorString(e));

@@ -732,21 +732,20 @@ template <typename T, bool AX, bool BX, int ACT, int BM, int BN, int WM, int WN,
 void launch_large(const Operand& a, const Operand& b, int64_t M, int64_t N, int64_t Kd, int64_t Ma,
                   int64_t Nb, int64_t parts, const Epilogue& e, float* ws, hipStream_t st) {
   const int64_t rows = ceil_div(M, BM), cols = ceil_div(N, BN), values = ROW_BYTES / sizeof(T);
-  TORCH_CHECK(rows * cols < (1LL << 31), "linear_act: too many tiles");
   const int64_t part = ceil_div(ceil_div(Kd, parts), values) * values;
   gemm_large_kernel<T, AX, BX, ACT, BM, BN, WM, WN, LB>
-      <<<dim3((unsigned)(rows * cols), (unsigned)parts), 64 * WM * WN, 0, st>>>(a, b, M, N, Kd, Ma, Nb, part,
-                                                                              rows, cols, e, ws);
+      <<<dim3(grid_of(rows * cols, 64 * WM * WN, "linear_act"), (unsigned)parts), 64 * WM * WN, 0, st>>>(
+          a, b, M, N, Kd, Ma, Nb, part, rows, cols, e, ws);
 }
 
 template <typename T, bool AX, bool BX, int ACT>
 void launch_small(const Operand& a, const Operand& b, int64_t M, int64_t N, int64_t Kd, int64_t parts,
                   const Epilogue& e, float* ws, hipStream_t st) {
   const int64_t rows = ceil_div(M, 64), cols = ceil_div(N, 64);
-  TORCH_CHECK(rows * cols < (1LL << 31), "linear_act: too many tiles");
   const int64_t part = ceil_div(ceil_div(Kd, parts), Tile<T>::BK) * Tile<T>::BK;
-  gemm_kernel<T, AX, BX, ACT, 64, 64><<<dim3((unsigned)(rows * cols), (unsigned)parts), NT, 0, st>>>(
-      a, b, M, N, Kd, part, cols, e, ws);
+  gemm_kernel<T, AX, BX, ACT, 64, 64>
+      <<<dim3(grid_of(rows * cols, NT, "linear_act"), (unsigned)parts), NT, 0, st>>>(a, b, M, N, Kd, part,
+                                                                                  cols, e, ws);
 }
 
 // Rows off the 16 bytes. Where they lie on 4, as fp32 always does, lanes load 4 bytes each: fp32
@@ -787,10 +786,9 @@ void gemm(const Tensor& a, const Tensor& b, int64_t M, int64_t N, int64_t Kd, co
       };
       Pad pa = pad(a, oa, fits_a, AX), pb = pad(b, ob, fits_b, BX);
       padded = at::empty({pa.rows * pa.ld + pb.rows * pb.ld}, like.options());
-      TORCH_CHECK(pa.rows + pb.rows < (1LL << 31), "linear_act: too many rows");
       pa.to = padded.data_ptr();
       pb.to = (char*)pa.to + pa.rows * pa.ld * elem;
-      MM_DISPATCH_TYPE(like, (pad_kernel<T><<<(unsigned)(pa.rows + pb.rows), NT, 0, st>>>(pa, pb)));
+      MM_DISPATCH_TYPE(like, (pad_kernel<T><<<grid_of(pa.rows + pb.rows, NT, "linear_act"), NT, 0, st>>>(pa, pb)));
       if (!fits_a) oa = {pa.to, pa.ld, true, true}, Ma = AX ? pa.ld : M;
       if (!fits_b) ob = {pb.to, pb.ld, true, true}, Nb = BX ? pb.ld : N;
       if (!fits_a && !fits_b) Kd = ceil_div(Kd, step) * step;
@@ -824,9 +822,8 @@ void gemm(const Tensor& a, const Tensor& b, int64_t M, int64_t N, int64_t Kd, co
         else
           launch_large<T, AX, BX, ACT, 64, 64, 2, 2>(oa, ob, M, N, Kd, Ma, Nb, c.parts, e, wp, st);
         if (c.parts > 1) {
-          TORCH_CHECK(ceil_div(M * N, NT) < (1LL << 31), "linear_act: too many values");
           join_kernel<T, ACT>
-              <<<(unsigned)ceil_div(M * N, NT), NT, 0, st>>>(wp, (int)c.parts, M * N, N, e);
+              <<<grid_of(ceil_div(M * N, NT), NT, "linear_act"), NT, 0, st>>>(wp, (int)c.parts, M * N, N, e);
         }
       }
     });
@@ -913,14 +910,13 @@ class LinearAct : public torch::autograd::Function<LinearAct> {
       const int64_t most = std::min<int64_t>(256, std::max<int64_t>(1, 2048 / cols));
       const int64_t chunk = M <= 128 ? M : std::max<int64_t>(16, ceil_div(M, most));
       const int64_t chunks = ceil_div(M, chunk);
-      TORCH_CHECK(cols * chunks < (1LL << 31), "linear_act: too many blocks");
       Tensor ws;
       const bool bias_float = need_b && db.scalar_type() == at::kFloat;
       if (need_b && chunks > 1) ws = at::empty({chunks * N}, dy.options().dtype(at::kFloat));
       float* wp = ws.defined() ? ws.data_ptr<float>() : nullptr;
       void* once = need_b && chunks == 1 ? db.data_ptr() : nullptr;
       MM_DISPATCH_TYPE(dy, MM_DISPATCH_ACT(act, {
-        act_bwd_kernel<T, ACT><<<(unsigned)(cols * chunks), NT, 0, st>>>(
+        act_bwd_kernel<T, ACT><<<grid_of(cols * chunks, NT, "linear_act"), NT, 0, st>>>(
             (const T*)ptr(dy), (const T*)ptr(saved[2]), M, N, cols, chunk, (T*)dz.data_ptr(), wp,
             once, bias_float);
       }));
