@@ -356,6 +356,7 @@ struct Tile {
   int tiles;      // of a sample
   int64_t blocks;
   unsigned int magic;  // for division by Cg
+  bool params;         // gamma and beta lie on 16 bytes
 };
 
 constexpr int MAX_WAVES = 16;
@@ -401,6 +402,19 @@ __device__ __forceinline__ void over_groups(const float* part, const Tile& t, in
   }
 }
 
+// The tile's means and 1/deviations, to memory and the latter to `spread` in the sums' place.
+__device__ __forceinline__ void tell_groups(const Tile& t, const Spot& p, float inv, float eps,
+                                            const float* group, float* spread, float* mean, float* rstd) {
+  for (int i = threadIdx.x; i < t.groups; i += blockDim.x) {
+    const int64_t at = p.n * t.G + p.tile * t.groups + i;
+    const float r = 1.f / sqrtf(spread[i] * inv + eps);
+    mean[at] = group[i] * inv;
+    rstd[at] = r;
+    spread[i] = r;
+  }
+  __syncthreads();
+}
+
 template <typename T, int V, int ACT, int KR>
 __global__ __launch_bounds__(1024) void gn_tile_kernel(
     const T* __restrict__ x, const T* __restrict__ res, Tile t, float eps, const void* __restrict__ gamma,
@@ -420,10 +434,9 @@ __global__ __launch_bounds__(1024) void gn_tile_kernel(
 #pragma unroll
   for (int i = 0; i < KR; ++i)
     if (p.active && p.row + i * p.step < t.R) val[i].load(x + first + i * stride);
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    ga[v] = load_param(gamma, p.c0 + (p.active ? p.col + v : 0), wf, 1.f);
-    be[v] = load_param(beta, p.c0 + (p.active ? p.col + v : 0), wf, 0.f);
+  if (p.active) {
+    load_params<V>(gamma, p.c0 + p.col, wf, t.params, 1.f, ga);
+    load_params<V>(beta, p.c0 + p.col, wf, t.params, 0.f, be);
   }
 #pragma unroll
   for (int i = 0; i < KR; ++i)
@@ -451,14 +464,10 @@ __global__ __launch_bounds__(1024) void gn_tile_kernel(
   __syncthreads();
   over_groups(part, t, pitch, spread);
   __syncthreads();
-  for (int i = threadIdx.x; i < t.groups; i += blockDim.x) {
-    const int64_t at = p.n * t.G + p.tile * t.groups + i;
-    mean[at] = group[i] * inv;
-    rstd[at] = 1.f / sqrtf(spread[i] * inv + eps);
-  }
+  tell_groups(t, p, inv, eps, group, spread, mean, rstd);
   if (!p.active) return;
 #pragma unroll
-  for (int v = 0; v < V; ++v) ga[v] *= 1.f / sqrtf(spread[g[v]] * inv + eps);
+  for (int v = 0; v < V; ++v) ga[v] *= spread[g[v]];
 #pragma unroll
   for (int i = 0; i < KR; ++i)
     if (p.row + i * p.step < t.R) {
@@ -543,11 +552,12 @@ __global__ __launch_bounds__(512) void gn_tile_bwd_kernel(
     for (int v = 0; v < V; ++v) {
       g[v] = p.active ? divided(p.col + v, t.magic) : 0;
       const int64_t at = p.n * t.G + p.tile * t.groups + g[v];
-      const int c = p.active ? p.c0 + p.col + v : p.c0;
       mu[v] = mean[at];
       rs[v] = rstd[at];
-      ga[v] = load_param(gamma, c, wf, 1.f);
-      be[v] = load_param(beta, c, wf, 0.f);
+    }
+    if (p.active) {
+      load_params<V>(gamma, p.c0 + p.col, wf, t.params, 1.f, ga);
+      load_params<V>(beta, p.c0 + p.col, wf, t.params, 0.f, be);
     }
 #pragma unroll
     for (int i = 0; i < KR; ++i)
@@ -651,18 +661,15 @@ __global__ __launch_bounds__(512, 4) void gn_stream_kernel(
   __syncthreads();
   over_groups(part, t, pitch, spread);
   __syncthreads();
-  for (int i = threadIdx.x; i < t.groups; i += blockDim.x) {
-    const int64_t at = p.n * t.G + p.tile * t.groups + i;
-    mean[at] = group[i] * inv;
-    rstd[at] = 1.f / sqrtf(spread[i] * inv + eps);
-  }
+  tell_groups(t, p, inv, eps, group, spread, mean, rstd);
   if (!p.active) return;
   float be[V];
+  load_params<V>(gamma, p.c0 + p.col, wf, t.params, 1.f, m2);
+  load_params<V>(beta, p.c0 + p.col, wf, t.params, 0.f, be);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     mu[v] = group[g[v]] * inv;
-    m2[v] = load_param(gamma, p.c0 + p.col + v, wf, 1.f) / sqrtf(spread[g[v]] * inv + eps);
-    be[v] = load_param(beta, p.c0 + p.col + v, wf, 0.f);
+    m2[v] *= spread[g[v]];
   }
   for (int64_t r = p.row, at = first; r < t.R; r += KR * p.step, at += KR * stride) {
     Packed<T, V> val[KR], rv[KR] = {};
@@ -704,11 +711,12 @@ __global__ __launch_bounds__(512, 4) void gn_stream_bwd_kernel(
   for (int v = 0; v < V; ++v) {
     g[v] = p.active ? divided(p.col + v, t.magic) : 0;
     const int64_t at = p.n * t.G + p.tile * t.groups + g[v];
-    const int c = p.active ? p.c0 + p.col + v : p.c0;
     mu[v] = mean[at];
     rs[v] = rstd[at];
-    ga[v] = load_param(gamma, c, wf, 1.f);
-    be[v] = load_param(beta, c, wf, 0.f);
+  }
+  if (p.active) {
+    load_params<V>(gamma, p.c0 + p.col, wf, t.params, 1.f, ga);
+    load_params<V>(beta, p.c0 + p.col, wf, t.params, 0.f, be);
   }
   // `with` gets each vector's place, xhat and dz
   const auto rows = [&](auto with) {
@@ -850,7 +858,7 @@ struct Plan {
 // 128x128x112x112 830 us by chunks, 600, 491 and 425 read twice in pieces of 32, 64 and 128;
 // 64x256x28x28 33 us held in 128, 53 read twice. Forward, 64x64x32x32: 11.4 us in pieces of 32 bytes
 // and 256 blocks, 13.5 in 16 and 512, 12.8 in 64 and 128; 128x256x56x56 141 held in 64, 198 in 32.
-Plan plan_of(const Image& im, int64_t groups, int V, int64_t elem, int max_threads, int most,
+Plan plan_of(const Image& im, int64_t groups, int V, int64_t elem, bool params, int max_threads, int most,
              double twice) {
   Plan best;
   double least = 1e30;
@@ -872,7 +880,7 @@ Plan plan_of(const Image& im, int64_t groups, int V, int64_t elem, int max_threa
                         std::max(1.0, 256.0 / blocks) * (rows ? 1.0 : twice);
     if (cost < least) {
       least = cost;
-      best.t = {im.R, im.C, G, Cg, k, lanes, G / k, blocks, magic_of(Cg)};
+      best.t = {im.R, im.C, G, Cg, k, lanes, G / k, blocks, magic_of(Cg), params};
       best.threads = rows ? threads : 512;
       best.rows = rows;
     }
@@ -930,7 +938,7 @@ void normalise(Forward& f, int64_t groups, double eps, int64_t act) {
   const bool wf = (w.defined() ? w : b.defined() ? b : x).scalar_type() == at::kFloat;
   const int vec = vector_of(im.C, x.element_size(), {ptr(x), ptr(res), ptr(y)});
   const hipStream_t st = stream_of(x);
-  const Plan plan = plan_of(im, groups, vec, x.element_size(), 1024, FWD_ROWS, 1.5);
+  const Plan plan = plan_of(im, groups, vec, x.element_size(), aligned({ptr(w), ptr(b)}, 16), 1024, FWD_ROWS, 1.5);
   if (plan.threads) {
     MM_DISPATCH_TYPE(x, GN_DISPATCH_TILE(vec, plan.rows, FWD_ROWS, MM_DISPATCH_ACT(act, (
         tile_of<T, V, ACT, KR>()<<<(unsigned)plan.t.blocks, plan.threads, 0, st>>>(
@@ -975,7 +983,7 @@ Grads backward_of(const Tensor& dy, const Tensor& x, int64_t groups, const Tenso
   const int vec = vector_of(im.C, x.element_size(),
                             {ptr(x), ptr(dy), ptr(res), ptr(g.dx), ptr(g.dres)});
   const hipStream_t st = stream_of(x);
-  const Plan plan = plan_of(im, groups, vec, x.element_size(), 512, BWD_ROWS, 1.15);
+  const Plan plan = plan_of(im, groups, vec, x.element_size(), aligned({ptr(w), ptr(b)}, 16), 512, BWD_ROWS, 1.15);
   Tensor ws;
   int64_t rows;  // of ws: what each sample, or each chunk of it, adds to the parameters' gradients
   if (plan.threads) {

@@ -52,11 +52,12 @@ template <typename T, int V>
 struct Packed {
   static constexpr int W = V * sizeof(T) / 4;
   unsigned int w[W];
+  static constexpr int ALIGNED = sizeof(T) * V < 16 ? sizeof(T) * V : 16;
   __device__ __forceinline__ void load(const T* p) {
-    *this = *(const Packed*)__builtin_assume_aligned(p, sizeof(T) * V);
+    *this = *(const Packed*)__builtin_assume_aligned(p, ALIGNED);
   }
   __device__ __forceinline__ void store(T* p) const {
-    *(Packed*)__builtin_assume_aligned(p, sizeof(T) * V) = *this;
+    *(Packed*)__builtin_assume_aligned(p, ALIGNED) = *this;
   }
   __device__ __forceinline__ float get(int i) const {
     if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
@@ -79,6 +80,28 @@ struct Packed {
 __device__ __forceinline__ float load_param(const void* p, int64_t i, bool is_float, float none) {
   if (p == nullptr) return none;
   return is_float ? ((const float*)p)[i] : to_float(((const bf16*)p)[i]);
+}
+// V of them from i on; `whole`: i and p allow whole vectors
+template <int V>
+__device__ __forceinline__ void load_params(const void* p, int64_t i, bool is_float, bool whole, float none,
+                                            float (&out)[V]) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) out[v] = none;
+  if (p == nullptr) return;
+  if (whole && is_float) {
+    Packed<float, V> q;
+    q.load((const float*)p + i);
+#pragma unroll
+    for (int v = 0; v < V; ++v) out[v] = q.get(v);
+  } else if (whole) {
+    Packed<bf16, V> q;
+    q.load((const bf16*)p + i);
+#pragma unroll
+    for (int v = 0; v < V; ++v) out[v] = q.get(v);
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) out[v] = load_param(p, i + v, is_float, none);
+  }
 }
 __device__ __forceinline__ void store_param(void* p, int64_t i, bool is_float, float v) {
   if (is_float)

@@ -414,6 +414,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_large_kernel(
   const auto up = [&](int at) { return lds + at * (2 * A::SIZE + B::SIZE); };
   const auto low = [&](int at) { return up(at) + A::SIZE; };
   const auto bs = [&](int at) { return up(at) + 2 * A::SIZE; };
+  if constexpr (AX || BX) e.bias = e.res = nullptr, e.z = nullptr;  // going back there are none
   int64_t tr, tc;
   tile_of(blockIdx.x, row_tiles, col_tiles, tr, tc);
   const int64_t m0 = tr * BM, n0 = tc * BN;
