@@ -2,9 +2,9 @@
 
 ``python -m murmura_amd.ops.build`` compiles the sources of hip/ with hipcc
 (one process a file, side by side) and links ``_murmura_hip.so`` next to this
-file so it travels to the GPU box with the repo snapshot (never a JIT cache
-under ~/.cache). hipcc cross-compiles without a GPU, so this runs in the
-CPU-only container too. The sources are HIP as they stand: they are handed to
+file, so that it goes wherever the tree goes (never a JIT cache under
+~/.cache). hipcc cross-compiles without a GPU, so this runs on a machine of
+CPUs too. The sources are HIP as they stand: they are handed to
 the compiler directly, with torch's include paths and defines.
 """
 

@@ -25,7 +25,7 @@ BF16, FP32 = torch.bfloat16, torch.float32
 
 @pytest.fixture(scope="module", autouse=True)
 def _require_native():
-    assert ops.native_available(), "HIP extension must be present on the GPU box"
+    assert ops.native_available(), "HIP extension must be present"
 
 
 def _half(dtype):
