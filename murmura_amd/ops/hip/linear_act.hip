@@ -934,7 +934,10 @@ class LinearAct : public torch::autograd::Function<LinearAct> {
     const Tensor b = bias.value_or(Tensor()), res = residual.value_or(Tensor());
     const bool need_x = x.requires_grad(), need_w = weight.requires_grad();
     const Forward f = forward_of(x, weight, b, res, act, true);
-    ctx->save_for_backward({need_w ? f.x : Tensor(), need_x ? f.w : Tensor(), f.keep});
+    // x itself and not the matrix that was made of it: a view made in here counts its changes by
+    // itself, and one in place would go unseen
+    const Tensor kept_x = f.x.is_alias_of(x) ? x : f.x;
+    ctx->save_for_backward({need_w ? kept_x : Tensor(), need_x ? f.w : Tensor(), f.keep});
     ctx->saved_data["act"] = act;
     ctx->saved_data["needs"] = (int64_t)(need_x | need_w << 1 | wants_grad(b) << 2 | wants_grad(res) << 3);
     ctx->saved_data["x"] = x.sizes().vec();
@@ -996,7 +999,7 @@ class LinearAct : public torch::autograd::Function<LinearAct> {
     if (needs & 2) {
       dw = at::empty({N, Kd}, dy.options());
       Epilogue e{nullptr, false, nullptr, nullptr, dw.data_ptr(), ACT_NONE, rows_of_8(Kd, {ptr(dw)})};
-      gemm<true, true>(dzm, saved[0], N, Kd, M, e, dy);
+      gemm<true, true>(dzm, saved[0].dim() == 2 ? saved[0] : saved[0].reshape({M, Kd}), N, Kd, M, e, dy);
     }
     return {dx, dw, db, needs & 8 ? dz : Tensor(), Tensor()};
   }
