@@ -271,7 +271,10 @@ def adamw_step(params: Union[Tensor, Sequence[Tensor]], grads: Union[Tensor, Seq
     which a captured step reads anew on each replay; the step's count too lives on
     the device. bf16 parameters and 8-bit moments are rounded up with the
     probability of what is cut off, by a hash of (seed, step, place): runs repeat
-    bit for bit, and ranks or nodes that shall differ take different seeds."""
+    bit for bit, and ranks or nodes that shall differ take different seeds.
+
+    A refused call leaves everything as it was. On a GPU, 8-bit moments refuse
+    over 160 tensors within 256 values: such small ones are passed as one."""
     params, grads = ref.as_list(params), ref.as_list(grads)
     if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
         raise ValueError(f"adamw_step: betas lie in [0, 1), got {betas}")

@@ -458,9 +458,6 @@ void adamw_step(const std::vector<Tensor>& params, std::vector<Tensor> grads,
                 "adamw_step: parameters share memory: pass each once");
   check_state(exp_avg, P, dev);
   check_state(exp_avg_sq, P, dev);
-  // a graph that saved a parameter must not be gone back through with its new values
-  for (const Tensor& p : params)
-    if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
   TORCH_CHECK(exp_avg.size() == exp_avg_sq.size(), "adamw_step: both moments in the same bits");
   TORCH_CHECK(step.device() == dev && step.scalar_type() == at::kLong && step.numel() == 1,
               "adamw_step: step is one int64 on the parameters' device");
@@ -490,14 +487,13 @@ void adamw_step(const std::vector<Tensor>& params, std::vector<Tensor> grads,
   h.lr_dev = lr_tensor.has_value() ? lr_tensor->data_ptr<float>() : nullptr;
   h.seed = (unsigned int)seed;
   h.step = step.data_ptr<int64_t>();
-  // 256 values with one scale must lie within one launch: a tensor that ends inside of them is
-  // listed again at the head of the next table.
-  size_t next = 0;
-  int64_t start = 0;  // place of params[next]
-  Table t;
-  t.begin = 0;
-  while (t.begin < P) {
+  // What a launch takes from place `begin` on, where params[next] holds it and starts at `start`. 256
+  // values with one scale must lie within one launch: a tensor that ends inside of them is listed
+  // again at the head of the next table.
+  const auto table_from = [&](int64_t begin, size_t& next, int64_t& start) {
+    Table t;
     t.count = 0;
+    t.begin = begin;
     int64_t at = start;
     size_t i = next;
     for (; i < params.size() && t.count < MAX_SEGMENTS; ++i) {
@@ -506,9 +502,29 @@ void adamw_step(const std::vector<Tensor>& params, std::vector<Tensor> grads,
       at += params[i].numel();
     }
     t.end = i == params.size() ? P : eight ? at / QB * QB : at;
-    TORCH_CHECK(t.end > t.begin, "adamw_step: over ", MAX_SEGMENTS, " tensors within ", QB,
-                " values of 8-bit moments: pass them as one");
     t.last = t.end == P;
+    while (next < i && start + params[next].numel() <= t.end) start += params[next++].numel();
+    return t;
+  };
+  // all that can be refused is refused before the first launch: a step is done as a whole or not at all
+  if (eight && params.size() > MAX_SEGMENTS) {
+    size_t next = 0;
+    int64_t start = 0;
+    for (int64_t begin = 0; begin < P;) {
+      const int64_t end = table_from(begin, next, start).end;
+      TORCH_CHECK(end > begin, "adamw_step: over ", MAX_SEGMENTS, " tensors within ", QB,
+                  " values of 8-bit moments: pass them as one");
+      begin = end;
+    }
+  }
+  // a graph that saved a parameter must not be gone back through with its new values
+  for (const Tensor& p : params)
+    if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+  size_t next = 0;
+  int64_t start = 0;
+  for (int64_t begin = 0; begin < P;) {
+    const Table t = table_from(begin, next, start);
+    begin = t.end;
     const int64_t chunks = ceil_div(t.end - t.begin, (int64_t)NT * 8);
     const int64_t blocks = std::min(chunks, chunks < (1 << 14) ? FEW_BLOCKS : MANY_BLOCKS);
     MM_DISPATCH_TYPE(params[0], {
@@ -521,9 +537,6 @@ void adamw_step(const std::vector<Tensor>& params, std::vector<Tensor> grads,
       }
     });
     check_launch("adamw_step");
-    // the next table starts with the tensor that holds place t.end
-    while (next < i && start + params[next].numel() <= t.end) start += params[next++].numel();
-    t.begin = t.end;
   }
   if (P == 0) step.add_(1);
 }

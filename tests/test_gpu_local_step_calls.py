@@ -38,3 +38,30 @@ def test_inputs_changed_in_place_are_noticed(lead, act):
     y = ops.linear_act(x, w, act=act)
     got, = torch.autograd.grad(y.sum(), w)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_adamw_refuses_before_it_changes_anything(bits):
+    """The refusal of a later launch, and of what is looked at last."""
+    def state(shapes):
+        p = [_randn(s, FP32, i).cuda() for i, s in enumerate(shapes)]
+        m, v, t = ops.adamw_state(sum(x.numel() for x in p), "cuda", bits)
+        return p, [torch.ones_like(x) for x in p], m, v, t
+
+    def refused(match, p, g, m, v, t, lr=1e-2):
+        moments = [x for moment in (m, v) for x in ([moment] if isinstance(moment, torch.Tensor) else moment)]
+        flat = [*p, *moments, t]
+        kept, versions = [x.clone() for x in flat], [x._version for x in p]
+        with pytest.raises(RuntimeError, match=match):
+            ops.adamw_step(p, g, m, v, t, lr)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(kept, flat))
+        assert versions == [x._version for x in p]
+
+    if bits == 8:  # 160 tensors fill the first launch, the next has over 160 within one scale
+        refused("pass them as one", *state([(4096,)] * 160 + [(1,)] * 200))
+    p, g, m, v, t = state([(300,), (20,)])
+    refused("int64", p, g, m, v, t.int())
+    refused("one fp32 value", p, g, m, v, t, torch.ones(2, device="cuda"))
+    refused("parameter", p, g, m, ops.adamw_state(321, "cuda", bits)[1], t)
+    refused("same bits", p, g, m, ops.adamw_state(320, "cuda", 40 - bits)[1], t)
