@@ -202,6 +202,14 @@ inline bool is_float_type(const Tensor& t) {
   return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16;
 }
 
+// A tensor that carries a derivative going forward would lose it without a word: the kernels know
+// none.
+inline void refuse_forward_mode(std::initializer_list<const Tensor*> inputs, const char* what) {
+  for (const Tensor* t : inputs)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), what,
+                ": no derivative going forward (forward-mode differentiation)");
+}
+
 inline unsigned int magic_of(int64_t d) {
   return (unsigned int)(((1LL << 32) + d - 1) / d);  // d = 1 gives 0
 }

@@ -2,6 +2,7 @@
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 pytestmark = pytest.mark.gpu
 
@@ -65,3 +66,18 @@ def test_adamw_refuses_before_it_changes_anything(bits):
     refused("one fp32 value", p, g, m, v, t, torch.ones(2, device="cuda"))
     refused("parameter", p, g, m, ops.adamw_state(321, "cuda", bits)[1], t)
     refused("same bits", p, g, m, ops.adamw_state(320, "cuda", 40 - bits)[1], t)
+
+
+def test_derivatives_going_forward_are_refused():
+    def duals(call, *args):
+        for i in range(len(args)):
+            with fwd.dual_level():
+                mixed = [fwd.make_dual(a, torch.ones_like(a)) if i == j else a for j, a in enumerate(args)]
+                for grad in (True, False):
+                    with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward"):
+                        call(*mixed)
+
+    x, w, b, r = (_randn(s, FP32, 1).cuda() for s in ((4, 8), (5, 8), (5,), (4, 5)))
+    duals(lambda x, w, b, r: ops.linear_act(x, w, b, res=r), x, w, b, r)
+    x, w, b, r = (_randn(s, FP32, 1).cuda() for s in ((2, 8, 3, 3), (8,), (8,), (2, 8, 3, 3)))
+    duals(lambda x, w, b, r: ops.group_norm_act(x, 2, w, b, res=r), x, w, b, r)
