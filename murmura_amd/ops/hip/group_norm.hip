@@ -1075,6 +1075,7 @@ Tensor group_norm_act(const Tensor& x, int64_t groups, const OptTensor& weight,
                res = residual.value_or(Tensor());
   check_args(x, groups, w, b, res, act);
   refuse_forward_mode({&x, &w, &b, &res}, "group_norm_act");
+  refuse_tracing("group_norm_act");
   const c10::DeviceGuard guard(x.device());
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b) || wants_grad(res)))
     return GroupNormAct::apply(x, weight, bias, residual, groups, eps, act);

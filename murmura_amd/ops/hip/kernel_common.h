@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 #include <ATen/ATen.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -208,6 +209,11 @@ inline void refuse_forward_mode(std::initializer_list<const Tensor*> inputs, con
   for (const Tensor* t : inputs)
     TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), what,
                 ": no derivative going forward (forward-mode differentiation)");
+}
+
+// A trace would hold the result's memory and not the kernels that fill it.
+inline void refuse_tracing(const char* what) {
+  TORCH_CHECK(!torch::jit::tracer::isTracing(), what, ": not to be traced (torch.jit.trace)");
 }
 
 inline unsigned int magic_of(int64_t d) {

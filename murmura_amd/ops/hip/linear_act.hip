@@ -1027,6 +1027,7 @@ Tensor linear_act(const Tensor& x, const Tensor& weight, const OptTensor& bias, 
   const c10::DeviceGuard guard(x.device());
   const Tensor b = bias.value_or(Tensor()), r = res.value_or(Tensor());
   refuse_forward_mode({&x, &weight, &b, &r}, "linear_act");
+  refuse_tracing("linear_act");
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(b) || wants_grad(r)))
     return LinearAct::apply(x, weight, bias, res, act);
   return forward_of(x, weight, b, r, act, false).y;

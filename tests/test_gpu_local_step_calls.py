@@ -81,3 +81,15 @@ def test_derivatives_going_forward_are_refused():
     duals(lambda x, w, b, r: ops.linear_act(x, w, b, res=r), x, w, b, r)
     x, w, b, r = (_randn(s, FP32, 1).cuda() for s in ((2, 8, 3, 3), (8,), (8,), (2, 8, 3, 3)))
     duals(lambda x, w, b, r: ops.group_norm_act(x, 2, w, b, res=r), x, w, b, r)
+
+
+def test_tracing_is_refused():
+    """A trace would hold the result's memory and not the kernel that fills it."""
+    from murmura_amd.ops.fused_linear import MurmuraLinear
+    from murmura_amd.ops.fused_norm import MurmuraGroupNorm
+
+    for module, x in ((MurmuraLinear(8, 5, act="relu"), _randn((3, 8), FP32, 1)),
+                      (MurmuraGroupNorm(2, 8), _randn((3, 8), FP32, 1))):
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="traced"):
+                torch.jit.trace(module.cuda(), x.cuda(), check_trace=False)
