@@ -117,9 +117,7 @@ class EvalContext:
         model = self.store.model
         batched = {}
         for e in spec.entries:
-            batched[e.name] = states[:, e.offset : e.offset + e.numel].view(
-                states.shape[0], *e.shape
-            )
+            batched[e.name] = self.store.stacked_view(states, e)
         shared = {
             name: b
             for name, b in model.named_buffers()

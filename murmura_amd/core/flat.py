@@ -119,6 +119,15 @@ class FlatParamStore:
             return sl.view(o, h, w, i).permute(0, 3, 1, 2)
         return sl.view(e.shape)
 
+    def stacked_view(self, states: Tensor, e: FlatEntry) -> Tensor:
+        """Entry ``e`` of k stacked flat states [k, P], in the order in which
+        this store holds it: [k, *shape]."""
+        sl = states[:, e.offset : e.offset + e.numel]
+        if self._is_nhwc(e):
+            o, i, h, w = e.shape
+            return sl.view(len(states), o, h, w, i).permute(0, 1, 4, 2, 3)
+        return sl.view(len(states), *e.shape)
+
     @torch.no_grad()
     def _write_entry(self, buf: Tensor, e: FlatEntry, src: Tensor) -> None:
         sl = buf[e.offset : e.offset + e.numel]

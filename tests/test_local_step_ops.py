@@ -239,3 +239,28 @@ def test_configuration_reaches_the_optimizer():
     model = factories.build_model_factory(
         Config(model={"factory": "models.resnet18", "params": {"norm": "group"}}))()
     assert isinstance(model.bn1, MurmuraGroupNorm)
+
+
+# --------------------------------------------- candidates scored in one pass
+def _scoring(model, shape, channels_last):
+    from murmura_amd.aggregation.base import EvalContext
+    from murmura_amd.core.flat import FlatParamStore
+
+    store = FlatParamStore(model, torch.device("cpu"), torch.float32, channels_last=channels_last)
+    data = TensorDataset(_randn(8, *shape, seed=9).float(), torch.arange(8) % 4)
+    context = EvalContext(store, DataLoader(data, batch_size=8), torch.device("cpu"))
+    base = store.snapshot()
+    return context, torch.stack([base, 0.9 * base, base + 0.01 * base.roll(1)])
+
+
+@pytest.mark.parametrize("channels_last", [False, True])
+@pytest.mark.parametrize("fused", [False, True])
+def test_candidates_in_channels_last_are_scored_as_one_by_one(channels_last, fused):
+    torch.manual_seed(0)
+    context, states = _scoring(FEMNISTModel(hidden=16, num_classes=4, fused=fused), (1, 28, 28), channels_last)
+    batch = context.next_batch()
+    got = context.losses_on_batch(states, batch)
+    assert context._vmap_ok is True
+    want = torch.stack([context.loss_on_batch(s, batch) for s in states])
+    # sums of up to 3136 products of values below 1, in another order
+    assert (got - want).abs().max() <= 3136 * 2.0 ** -24
