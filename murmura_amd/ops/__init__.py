@@ -221,6 +221,52 @@ def scale_inject(flat: Tensor, lam: float) -> Tensor:
     return ref.scale_inject(flat, lam)
 
 
+# ------------------------------------------------- under torch.vmap (K16, K18)
+def _is_mapped(*tensors: Optional[Tensor]) -> bool:
+    """Whether torch.vmap is at work on one of them: those have no memory that a kernel could read."""
+    if not torch._C._are_functorch_transforms_active():
+        return False
+    functorch = torch._C._functorch
+    return functorch.peek_interpreter_stack().key() == functorch.TransformType.Vmap and any(
+        t is not None and functorch.is_batchedtensor(t) for t in tensors)
+
+
+def _one_by_one(op, info, in_dims, args):
+    """The mapped call as one call for each element, so that each has the results that it has alone."""
+    return torch.stack([
+        op(*(a if d is None else a.select(d, i) for a, d in zip(args, in_dims)))
+        for i in range(info.batch_size)
+    ]), 0
+
+
+class _MappedGroupNormAct(torch.autograd.Function):
+    @staticmethod
+    def forward(x, num_groups, weight, bias, eps, act, res):
+        return group_norm_act(x, num_groups, weight, bias, eps, act, res)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        pass
+
+    @staticmethod
+    def vmap(info, in_dims, *args):
+        return _one_by_one(group_norm_act, info, in_dims, args)
+
+
+class _MappedLinearAct(torch.autograd.Function):
+    @staticmethod
+    def forward(x, weight, bias, act, res):
+        return linear_act(x, weight, bias, act, res)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        pass
+
+    @staticmethod
+    def vmap(info, in_dims, *args):
+        return _one_by_one(linear_act, info, in_dims, args)
+
+
 # ------------------------------------------------------------------ K16
 def group_norm_act(x: Tensor, num_groups: int, weight: Optional[Tensor] = None,
                    bias: Optional[Tensor] = None, eps: float = 1e-5, act: str = "none",
@@ -232,9 +278,12 @@ def group_norm_act(x: Tensor, num_groups: int, weight: Optional[Tensor] = None,
     last (another layout is copied first) and y comes back so. weight and bias
     ([C]) are of x's type or fp32, res is like x. act: "none", "relu", "silu"
     or "gelu" (by erf). Statistics are held in fp32 and belong to each sample
-    alone: nothing is kept between calls."""
+    alone: nothing is kept between calls. Under torch.vmap each element is a
+    call; other transforms, and a derivative going forward, are refused on a GPU."""
     ref.check_group_norm_act(x, num_groups, weight, bias, res)
     code = ref.check_act(act)
+    if _is_mapped(x, weight, bias, res):
+        return _MappedGroupNormAct.apply(x, num_groups, weight, bias, eps, act, res)
     if _use_native(x):
         return _EXT.group_norm_act(x, num_groups, weight, bias, eps, code, res)
     return ref.group_norm_act(x, num_groups, weight, bias, eps, act, res)
@@ -308,9 +357,13 @@ def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: st
     x is [..., K], weight [N, K] (``nn.Linear``'s layout), fp32 or bf16, of one
     type; bias [N] of that type or fp32; res like y. act: "none", "relu",
     "silu" or "gelu" (by erf). Sums are fp32, also over bf16 products. For the
-    backward pass silu and gelu keep what they are taken of, in x's type."""
+    backward pass silu and gelu keep what they are taken of, in x's type. Under
+    torch.vmap, on a GPU, each element is a call; other transforms, and a
+    derivative going forward, are refused there."""
     ref.check_linear_act(x, weight, bias, res)
     code = ref.check_act(act)
     if _use_native(x):
+        if _is_mapped(x, weight, bias, res):
+            return _MappedLinearAct.apply(x, weight, bias, act, res)
         return _EXT.linear_act(x, weight, bias, code, res)
     return ref.linear_act(x, weight, bias, act, res)

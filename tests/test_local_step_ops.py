@@ -264,3 +264,44 @@ def test_candidates_in_channels_last_are_scored_as_one_by_one(channels_last, fus
     want = torch.stack([context.loss_on_batch(s, batch) for s in states])
     # sums of up to 3136 products of values below 1, in another order
     assert (got - want).abs().max() <= 3136 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("channels_last", [False, True])
+def test_candidates_with_group_norm_are_scored_in_one_pass(channels_last):
+    torch.manual_seed(0)
+    context, states = _scoring(ResNet18(num_classes=4, norm="group", groups=8), (3, 8, 8), channels_last)
+    batch = context.next_batch()
+    got = context.losses_on_batch(states, batch)
+    assert context._vmap_ok is True
+    want = torch.stack([context.loss_on_batch(s, batch) for s in states])
+    # 20 layers of sums of up to 4608 products
+    assert (got - want).abs().max() <= 20 * 4608 * 2.0 ** -24
+
+
+def test_operators_under_vmap():
+    x, w, b = (_randn(*s, seed=i) for i, s in enumerate(((3, 4, 8), (3, 5, 8), (3, 5))))
+
+    def f(x, w, b):
+        return ops.linear_act(x, w, b, "silu")
+
+    want = torch.stack([f(*t) for t in zip(x, w, b)])
+    assert torch.allclose(torch.vmap(f)(x, w, b), want, rtol=0, atol=64 * 2.0 ** -53 * 64)
+    x, w, r = (_randn(*s, seed=i) for i, s in enumerate(((3, 2, 8, 3, 5), (3, 8), (2, 8, 3, 5))))
+
+    def n(x, w):
+        return ops.group_norm_act(x, 2, w, act="relu", res=r)
+
+    want = torch.stack([n(*t) for t in zip(x, w)])
+    assert torch.equal(torch.vmap(n)(x, w), want)
+    assert torch.equal(torch.vmap(n, (None, 0))(x[0], w)[0], want[0])
+    pairs = torch.vmap(torch.vmap(n, (None, 0)), (0, None))(x, w)
+    assert torch.equal(torch.stack([pairs[i, i] for i in range(3)]), want)
+    assert torch.vmap(lambda w: (w * n(x[0], torch.ones(8).double()).sum()))(w).shape == w.shape
+    # gradients, of what is mapped over and of what is not
+    leaves = [t.clone().requires_grad_(True) for t in (x, w)]
+    got = torch.autograd.grad(torch.vmap(n)(*leaves).square().sum(), leaves)
+    again = torch.autograd.grad(torch.stack([n(*t) for t in zip(*leaves)]).square().sum(), leaves)
+    assert all(torch.equal(p, q) for p, q in zip(got, again))
+    # other transforms go through the plain operations
+    assert torch.allclose(torch.func.grad(lambda w: n(x[0], w).sum())(w[0]),
+                          torch.autograd.grad(n(x[0], leaves[1][0]).sum(), leaves[1])[0][0])
