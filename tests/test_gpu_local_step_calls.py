@@ -109,12 +109,12 @@ def _scoring(model, shape, device, dtype=FP32, channels_last=True, classes=4):
     return context, torch.stack([base, 0.9 * base, base + 0.01 * base.roll(1)])
 
 
-@pytest.mark.parametrize("name", ["mlp", "wide", "femnist", "resnet"])
+@pytest.mark.parametrize("name", ["mlp", "wide", "femnist"])
 def test_candidates_are_scored_in_one_graph(name):
     """All candidates through one captured, mapped forward, as without the fused layers, and as one
     by one: the fused layers run the same kernels, convolutions sum in another order (2^-24 times
-    some thousand products, over 20 layers in the ResNet, of a loss below 10)."""
-    from murmura_amd.models import FEMNISTModel, ResNet18, SimpleMLP
+    some thousand products, of a loss below 10)."""
+    from murmura_amd.models import FEMNISTModel, SimpleMLP
     from murmura_amd.models.zoo import WideMLP
 
     torch.manual_seed(0)
@@ -122,7 +122,6 @@ def test_candidates_are_scored_in_one_graph(name):
         "mlp": (lambda: SimpleMLP(12, fused=True), (12,), 64 * U),
         "wide": (lambda: WideMLP(12, 40, 4, fused=True), (12,), 64 * U),
         "femnist": (lambda: FEMNISTModel(hidden=64, num_classes=4, fused=True), (1, 28, 28), 4000 * U),
-        "resnet": (lambda: ResNet18(num_classes=4, norm="group"), (3, 16, 16), 20 * 4000 * U),
     }[name]
     context, states = _scoring(model(), shape, "cuda")
     batch = context.next_batch()
@@ -132,6 +131,22 @@ def test_candidates_are_scored_in_one_graph(name):
         want = torch.stack([context.loss_on_batch(s, batch) for s in states])
         assert (got - want).abs().max() <= 10 * tol
         states = states.flip(0)
+
+
+def test_candidates_with_group_norm_are_scored_one_by_one():
+    """Which is faster (what each measured stands at EvalContext), and the same losses."""
+    from murmura_amd.models import ResNet18
+
+    torch.manual_seed(0)
+    context, states = _scoring(ResNet18(num_classes=4, norm="group"), (3, 16, 16), "cuda")
+    batch = context.next_batch()
+    got = context.losses_on_batch(states, batch)
+    assert context._vmap_ok is False and not context._graphs
+    x, y = batch[0].contiguous(memory_format=torch.channels_last), batch[1]
+    with torch.no_grad():
+        mapped = context._ce_from_logits(context._stacked_call(states, x), y)
+    # 20 layers of sums of up to 4608 products, of a loss below 10
+    assert (got - mapped).abs().max() <= 10 * 20 * 4608 * U
 
 
 def test_operators_under_vmap(device="cuda"):
