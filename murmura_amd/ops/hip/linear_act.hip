@@ -317,7 +317,10 @@ struct Direct {
       at[i] = (unsigned)(ACROSS ? k * o.ld + r : r * o.ld + k) * sizeof(T);
     }
   }
-  // `wave` the same for all lanes
+  // `wave` the same for all lanes. m0, which the load reads and the compiler sets for its own uses
+  // alone, is told as overwritten; that it is not kept for anybody is what the warning says.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
   __device__ __forceinline__ void load(T* lds, int wave) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
@@ -326,15 +329,16 @@ struct Direct {
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                      :
                      : "s"(to), "v"(at[i]), "s"(base)
-                     : "memory");
+                     : "memory", "m0");
       else
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
                      :
                      : "s"(to), "v"(at[i]), "s"(base)
-                     : "memory");
+                     : "memory", "m0");
     }
     base += step;
   }
+#pragma clang diagnostic pop
   // the `left` values of k behind `steps` whole tiles
   __device__ __forceinline__ void load_tail(T* lds, int64_t steps, int left) const {
     const T* p = base + steps * step;
