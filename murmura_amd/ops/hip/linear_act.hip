@@ -732,12 +732,14 @@ struct Pad {
 
 template <typename T>
 __global__ __launch_bounds__(NT) void pad_kernel(Pad a, Pad b) {
-  const bool second = (int64_t)blockIdx.x >= a.rows;
-  const Pad& p = second ? b : a;
-  const int64_t row = second ? blockIdx.x - a.rows : blockIdx.x;
-  const T* from = (const T*)p.from.p + row * p.from.ld;
-  T* to = (T*)p.to + row * p.ld;
-  for (int64_t c = threadIdx.x; c < p.ld; c += NT) to[c] = row < p.full && c < p.cols ? from[c] : T{};
+  for (int64_t i = blockIdx.x; i < a.rows + b.rows; i += gridDim.x) {
+    const bool second = i >= a.rows;
+    const Pad& p = second ? b : a;
+    const int64_t row = second ? i - a.rows : i;
+    const T* from = (const T*)p.from.p + row * p.from.ld;
+    T* to = (T*)p.to + row * p.ld;
+    for (int64_t c = threadIdx.x; c < p.ld; c += NT) to[c] = row < p.full && c < p.cols ? from[c] : T{};
+  }
 }
 
 struct Choice {
@@ -851,7 +853,9 @@ void gemm(const Tensor& a, const Tensor& b, int64_t M, int64_t N, int64_t Kd, co
       padded = at::empty({pa.rows * pa.ld + pb.rows * pb.ld}, like.options());
       pa.to = padded.data_ptr();
       pb.to = (char*)pa.to + pa.rows * pa.ld * elem;
-      MM_DISPATCH_TYPE(like, (pad_kernel<T><<<grid_of(pa.rows + pb.rows, NT, "linear_act"), NT, 0, st>>>(pa, pb)));
+      // a block a row, as far as a launch has blocks
+      const unsigned rows = (unsigned)std::min<int64_t>(pa.rows + pb.rows, 1 << 20);
+      MM_DISPATCH_TYPE(like, (pad_kernel<T><<<rows, NT, 0, st>>>(pa, pb)));
       if (!fits_a) oa = {pa.to, pa.ld, true, true}, Ma = AX ? pa.ld : M;
       if (!fits_b) ob = {pb.to, pb.ld, true, true}, Nb = BX ? pb.ld : N;
       if (!fits_a && !fits_b) Kd = ceil_div(Kd, step) * step;

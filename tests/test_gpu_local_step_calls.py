@@ -9,7 +9,7 @@ pytestmark = pytest.mark.gpu
 from murmura_amd import ops
 
 U = 2.0 ** -24
-FP32 = torch.float32
+BF16, FP32 = torch.bfloat16, torch.float32
 
 
 def _randn(shape, dtype, seed):
@@ -176,3 +176,19 @@ def test_operators_under_vmap(device="cuda"):
     want = torch.stack([n(*t) for t in zip(x, w)])
     assert torch.equal(torch.vmap(n)(x, w), want)
     assert torch.equal(torch.vmap(n, (None, 0))(x[0], w)[0], want[0])
+
+
+def test_linear_over_more_rows_than_a_launch_has_blocks():
+    """2^24 + 3 odd rows of bf16. All values are -1, 0 or 1, so that every sum is a whole number
+    that fp32 holds: results are exact but for their own rounding."""
+    m, k, n = 2 ** 24 + 3, 9, 8
+    g = torch.Generator("cuda").manual_seed(1)
+    x, w, dy = (torch.randint(-1, 2, s, generator=g, device="cuda").to(BF16) for s in ((m, k), (n, k), (m, n)))
+    x, w = x.requires_grad_(True), w.requires_grad_(True)
+    y = ops.linear_act(x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    for rows in (slice(0, 1000), slice(m // 2, m // 2 + 1000), slice(m - 1000, m)):
+        assert torch.equal(y[rows].float(), (x[rows].float() @ w.float().t()).to(BF16).float())
+        assert torch.equal(dx[rows].float(), (dy[rows].float() @ w.float()).to(BF16).float())
+    want = torch.stack([(dy * x[:, i:i + 1]).to(torch.int32).sum(0) for i in range(k)], 1)
+    assert want.abs().max() < 2 ** 24 and torch.equal(dw, want.float().to(BF16))
