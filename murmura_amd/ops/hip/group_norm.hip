@@ -204,7 +204,7 @@ __global__ __launch_bounds__(NT) void gn_apply_kernel(
     for (int v = 0; v < V; ++v) {
       float z = a.xhat(to_float(xv.e[v]), v) * a.ga[v] + a.be[v];
       if (res) z += to_float(rv.e[v]);
-      yv.e[v] = from_float<T>(act_fwd<ACT>(z));
+      yv.e[v] = from_float<T>(act_fwd<T, ACT>(z));
     }
     *(Vec<T, V>*)(y + at) = yv;
   }
@@ -237,7 +237,7 @@ __global__ __launch_bounds__(NT) void gn_bwd_sums_kernel(
         const float xh = a.xhat(to_float(xv.e[v]), v);
         float z = xh * a.ga[v] + a.be[v];
         if (res) z += to_float(rv.e[v]);
-        const float dz = act_bwd<ACT>(to_float(dv.e[v]), z);
+        const float dz = act_bwd<T, ACT>(to_float(dv.e[v]), z);
         sz[v] += dz;
         sx[v] += dz * xh;
         dr.e[v] = from_float<T>(dz);
@@ -308,7 +308,7 @@ __global__ __launch_bounds__(NT) void gn_bwd_dx_kernel(
       const float xh = a.xhat(to_float(xv.e[v]), v);
       float z = xh * a.ga[v] + a.be[v];
       if (res) z += to_float(rv.e[v]);
-      const float dz = act_bwd<ACT>(to_float(dv.e[v]), z);
+      const float dz = act_bwd<T, ACT>(to_float(dv.e[v]), z);
       out.e[v] = from_float<T>(a.rs[v] * (dz * a.ga[v] - m[v].x - xh * m[v].y));
     }
     *(Vec<T, V>*)(dx + at) = out;
@@ -476,7 +476,7 @@ __global__ __launch_bounds__(1024) void gn_tile_kernel(
       float z[V];
 #pragma unroll
       for (int v = 0; v < V; ++v)
-        z[v] = act_fwd<ACT>((val[i].get(v) - mu[v]) * ga[v] + be[v] + r.get(v));
+        z[v] = act_fwd<T, ACT>((val[i].get(v) - mu[v]) * ga[v] + be[v] + r.get(v));
 #pragma unroll
       for (int v = 0; v < V / 2; ++v) o.set2(v, z[2 * v], z[2 * v + 1]);
       o.store(y + first + i * stride);
@@ -567,7 +567,7 @@ __global__ __launch_bounds__(512) void gn_tile_bwd_kernel(
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           const float xh = (xv[i].get(v) - mu[v]) * rs[v];
-          dz[i][v] = act_bwd<ACT>(dz[i][v], xh * ga[v] + be[v] + r.get(v));
+          dz[i][v] = act_bwd<T, ACT>(dz[i][v], xh * ga[v] + be[v] + r.get(v));
           sz[v] += dz[i][v];
           sx[v] += dz[i][v] * xh;
         }
@@ -685,7 +685,7 @@ __global__ __launch_bounds__(512, 4) void gn_stream_kernel(
         float z[V];
 #pragma unroll
         for (int v = 0; v < V; ++v)
-          z[v] = act_fwd<ACT>((val[i].get(v) - mu[v]) * m2[v] + be[v] + rv[i].get(v));
+          z[v] = act_fwd<T, ACT>((val[i].get(v) - mu[v]) * m2[v] + be[v] + rv[i].get(v));
 #pragma unroll
         for (int v = 0; v < V / 2; ++v) val[i].set2(v, z[2 * v], z[2 * v + 1]);
         val[i].store(y + at + i * stride);
@@ -737,7 +737,7 @@ __global__ __launch_bounds__(512, 4) void gn_stream_bwd_kernel(
 #pragma unroll
           for (int v = 0; v < V; ++v) {
             xh[v] = (xv[i].get(v) - mu[v]) * rs[v];
-            dz[v] = act_bwd<ACT>(dv[i].get(v), xh[v] * ga[v] + be[v] + rv[i].get(v));
+            dz[v] = act_bwd<T, ACT>(dv[i].get(v), xh[v] * ga[v] + be[v] + rv[i].get(v));
           }
           with(at + i * stride, xh, dz);
         }

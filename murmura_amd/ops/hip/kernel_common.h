@@ -146,49 +146,88 @@ __device__ __forceinline__ int divided(int a, unsigned int magic) {
 // ------------------------------------------------------------- activations
 enum Act { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3 };
 
-// Exponential and reciprocal are the hardware's, within one unit in the last place: an exact
-// division alone would take more instructions than all of the rest.
+// Exponential and reciprocal are the hardware's, within one unit in the last place. For fp32 what
+// the exponent's rounding cuts off is put back, so that the whole stays within 2^-22; for bf16, where a
+// result is rounded by 2^-8 of itself, exp(-x) may be off by 2^-24 |x|.
+__device__ __forceinline__ float exp2_of(float y, float rest) {  // 2^(y + rest)
+  return __builtin_amdgcn_exp2f(y) * __builtin_fmaf(rest, 0.69314718055994531f, 1.f);
+}
+template <typename T>
 __device__ __forceinline__ float exp_neg(float x) {  // exp(-x)
-  return __builtin_amdgcn_exp2f(x * -1.44269504088896341f);
+  constexpr float C = -1.44269504088896341f, LOW = -1.92596299e-8f;  // C in fp32 and its rest
+  if constexpr (sizeof(T) == 4) {
+    x = __builtin_amdgcn_fmed3f(x, -104.f, 104.f);  // beyond, it is infinite or zero
+    const float y = x * C;
+    return exp2_of(y, __builtin_fmaf(x, LOW, __builtin_fmaf(x, C, -y)));
+  }
+  return __builtin_amdgcn_exp2f(x * C);
 }
+template <typename T>
 __device__ __forceinline__ float sigmoid(float z) {
-  return __builtin_amdgcn_rcpf(1.f + exp_neg(z));
+  return __builtin_amdgcn_rcpf(1.f + exp_neg<T>(z));
 }
-// The normal distribution at z, and exp(-z*z/2), which its density shares with it: erfc by
-// Abramowitz and Stegun, 7.1.26, within 1.5e-7.
+// The normal distribution at z, and exp(-z*z/2), which its density shares with it.
+//
+// For fp32: erfc(a) = t P(t) exp(-a*a) with t = 1 / (1 + 0.3 a) and P of degree 8, fitted to least
+// relative error over 0 <= a <= 10, 2.0e-8. The square's rounding is left: gelu is within 9 + z*z/2
+// times 2^-24 of itself, its rms error over normal z 4.2e-8 (by erf in fp32 3.7e-8).
+// For bf16: erfc by Abramowitz and Stegun, 7.1.26, within 1.5e-7 (5e-5 of itself at z = -3), with which
+// fp32 would have 8.6e-8. Group norm over 64x128x56x56 in fp32 with gelu takes 50 us forward and 94 back,
+// with that form 46 and 93, with the math library's erfc and exp 66 and 130; with silu 2% more than
+// by the short exponential.
+template <typename T>
 __device__ __forceinline__ float normal_cdf(float z, float& e) {
-  const float a = fabsf(z) * 0.70710678118654752f;
-  const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * a);
-  e = exp_neg(a * a);
-  const float poly =
-      t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-  const float half = 0.5f * poly * e;
+  float half;
+  if constexpr (sizeof(T) == 4) {
+    constexpr float C = -0.72134752044448170f;  // -log2(e)/2
+    const float a = fminf(fabsf(z), 15.f);  // beyond, it is 0 or 1
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(a, 0.212132034f, 1.f));
+    const float square = a * a, y = square * C;
+    e = exp2_of(y, __builtin_fmaf(square, C, -y));
+    float p = -0.0647613704f;  // P / 2
+    p = __builtin_fmaf(p, t, 0.242781207f);
+    p = __builtin_fmaf(p, t, -0.256138206f);
+    p = __builtin_fmaf(p, t, 0.273859084f);
+    p = __builtin_fmaf(p, t, -0.0473247133f);
+    p = __builtin_fmaf(p, t, 0.107462756f);
+    p = __builtin_fmaf(p, t, 0.0741696581f);
+    p = __builtin_fmaf(p, t, 0.0853576064f);
+    p = __builtin_fmaf(p, t, 0.0845940039f);
+    half = p * t * e;
+  } else {
+    const float a = fabsf(z) * 0.70710678118654752f;
+    const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * a);
+    e = exp_neg<T>(a * a);
+    const float poly =
+        t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+    half = 0.5f * poly * e;
+  }
   return z < 0.f ? half : 1.f - half;
 }
 
-// act(z). A NaN stays one in each of them.
-template <int ACT>
+// act(z), for results of type T. A NaN stays one in each of them.
+template <typename T, int ACT>
 __device__ __forceinline__ float act_fwd(float z) {
   if constexpr (ACT == ACT_RELU) return z < 0.f ? 0.f : z;
-  if constexpr (ACT == ACT_SILU) return z * sigmoid(z);
+  if constexpr (ACT == ACT_SILU) return z * sigmoid<T>(z);
   if constexpr (ACT == ACT_GELU) {
     float e;
-    return z * normal_cdf(z, e);
+    return z * normal_cdf<T>(z, e);
   }
   return z;
 }
 
 // dy * act'(z)
-template <int ACT>
+template <typename T, int ACT>
 __device__ __forceinline__ float act_bwd(float dy, float z) {
   if constexpr (ACT == ACT_RELU) return z <= 0.f ? 0.f : dy;
   if constexpr (ACT == ACT_SILU) {
-    const float s = sigmoid(z);
+    const float s = sigmoid<T>(z);
     return dy * (s * (1.f + z * (1.f - s)));
   }
   if constexpr (ACT == ACT_GELU) {
     float e;
-    const float cdf = normal_cdf(z, e);
+    const float cdf = normal_cdf<T>(z, e);
     return dy * (cdf + z * (e * 0.39894228040143268f));
   }
   return dy;

@@ -43,7 +43,7 @@ template <typename T, int ACT>
 __device__ __forceinline__ void finish(const Epilogue& e, int64_t at, float v, float bias, float res) {
   const float z = v + bias + res;
   if (e.z) ((T*)e.z)[at] = from_float<T>(z);
-  ((T*)e.out)[at] = from_float<T>(act_fwd<ACT>(z));
+  ((T*)e.out)[at] = from_float<T>(act_fwd<T, ACT>(z));
 }
 
 template <typename T>
@@ -79,7 +79,7 @@ __device__ __forceinline__ void finish8(const Epilogue& e, int64_t at, const flo
     o.store(e.z, at);
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) o[i] = from_float<T>(act_fwd<ACT>(z[i]));
+  for (int i = 0; i < 8; ++i) o[i] = from_float<T>(act_fwd<T, ACT>(z[i]));
   o.store(e.out, at);
 }
 
@@ -615,7 +615,7 @@ __global__ __launch_bounds__(NT) void act_bwd_kernel(const T* __restrict__ dy,
       const int64_t at = r * N + c;
       float d = to_float(dy[at]);
       if constexpr (ACT != ACT_NONE) {
-        d = act_bwd<ACT>(d, to_float(z[at]));
+        d = act_bwd<T, ACT>(d, to_float(z[at]));
         dz[at] = from_float<T>(d);
       }
       s += d;
@@ -662,7 +662,7 @@ __global__ __launch_bounds__(NT) void act_bwd_vector_kernel(const T* __restrict_
 #pragma unroll
           for (int v = 0; v < V; ++v) {
             g[v] = d[i].get(v);
-            if constexpr (ACT != ACT_NONE) g[v] = act_bwd<ACT>(g[v], x[i].get(v));
+            if constexpr (ACT != ACT_NONE) g[v] = act_bwd<T, ACT>(g[v], x[i].get(v));
             s[v] += g[v];
           }
           if constexpr (ACT != ACT_NONE) {

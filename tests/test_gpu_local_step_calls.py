@@ -1,5 +1,7 @@
 """Calls of the local training step's operators beside the ordinary ones."""
 
+import math
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
@@ -15,6 +17,13 @@ BF16, FP32 = torch.bfloat16, torch.float32
 def _randn(shape, dtype, seed):
     g = torch.Generator().manual_seed(seed)
     return torch.randn(shape, generator=g, dtype=torch.float64).to(dtype)
+
+
+def _within(got, want, tol):
+    err = (got.double().cpu() - want).abs()
+    worst = (err - tol).max().item()
+    assert got.shape == want.shape
+    assert worst <= 0, f"off by {worst:.3g} more than allowed (error {err.max().item():.3g})"
 
 
 @pytest.mark.parametrize("lead", [(), (6,), (2, 3), (2, 1, 4)])
@@ -192,3 +201,30 @@ def test_linear_over_more_rows_than_a_launch_has_blocks():
         assert torch.equal(dx[rows].float(), (dy[rows].float() @ w.float()).to(BF16).float())
     want = torch.stack([(dy * x[:, i:i + 1]).to(torch.int32).sum(0) for i in range(k)], 1)
     assert want.abs().max() < 2 ** 24 and torch.equal(dw, want.float().to(BF16))
+
+
+def test_activations_in_fp32_hold_its_bits():
+    """z * 1 is z, so y and dx are the activation and its derivative alone.
+
+    erfc is within 4 units (8 u), its argument |z| sqrt(1/2) within 2 u, by which erfc changes at
+    most z^2 + 1 times as much; exp within 1 unit, its argument z^2/2 within u; the reciprocal
+    within 1 unit; a few products and sums of u each."""
+    z = torch.cat([torch.linspace(-9, 9, 20011), torch.linspace(-80, 80, 20011)])
+    x, one = z.view(-1, 1).cuda().requires_grad_(True), torch.ones(1, 1, device="cuda")
+    for act in ("silu", "gelu"):
+        y = ops.linear_act(x, one, act=act)
+        dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+        d = z.double()
+        if act == "silu":
+            s, c = torch.sigmoid(d), torch.sigmoid(-d)
+            t = 1 + d * c
+            _within(y.detach().view(-1), d * s, 8 * U * (d * s).abs())
+            _within(dx.view(-1), s * t, U * s * (8 * d.abs() + 2 + 8 * t.abs()))
+            continue
+        near = d.abs() <= 9  # beyond, erfc leaves the normal numbers
+        cdf, pdf = 0.5 * torch.erfc(-d * math.sqrt(0.5)), torch.exp(-0.5 * d * d) / math.sqrt(2 * math.pi)
+        _within(y.detach().view(-1)[near], (d * cdf)[near], U * ((2 * d * d + 12) * (d * cdf).abs())[near])
+        _within(dx.view(-1)[near], (cdf + d * pdf)[near],
+                U * ((2 * d * d + 12) * cdf + d.abs() * pdf * (d * d + 8))[near])
+        assert torch.equal(y.detach().view(-1)[z.cuda() > 9], z.cuda()[z.cuda() > 9])
+        assert y.detach().view(-1)[z.cuda() < -9].abs().max() < 1e-17
