@@ -25,6 +25,7 @@ struct Operand {
   int64_t ld;  // values from one row in memory to the next
   bool whole;  // rows and base allow 16-byte loads
   bool words;  // or 4-byte ones
+  const void* rest;  // what p's values were rounded by, laid out like them, or null
 };
 
 struct Epilogue {
@@ -155,8 +156,9 @@ struct Stage {
 };
 
 // Four waves side by side two by two, each with (BM/2) x (BN/2) of the tile in 16x16 blocks. A
-// lane holds 4 rows of one column of each block.
-template <typename T, bool AX, bool BX, int ACT, int BM, int BN>
+// lane holds 4 rows of one column of each block. HALVES: how often the sum is gone over, twice where A
+// comes in two halves, of which the rest is the second.
+template <typename T, bool AX, bool BX, int ACT, int BM, int BN, int HALVES>
 __global__ __launch_bounds__(NT) void gemm_kernel(Operand a, Operand b, int64_t M, int64_t N,
                                                   int64_t Kd, int64_t k_part, int64_t col_tiles,
                                                   Epilogue e, float* __restrict__ ws) {
@@ -175,47 +177,50 @@ __global__ __launch_bounds__(NT) void gemm_kernel(Operand a, Operand b, int64_t 
     for (int j = 0; j < FN; ++j) acc[i][j] = {0.f, 0.f, 0.f, 0.f};
   Stage<T, AX, BM> sa;
   Stage<T, BX, BN> sb;
-  if (kb < ke) {
-    sa.load(a, m0, kb, M, ke);
-    sb.load(b, n0, kb, N, ke);
-  }
-  for (int64_t k0 = kb; k0 < ke; k0 += BK) {
-    sa.store(as);
-    sb.store(bs);
-    __syncthreads();
-    if (k0 + BK < ke) {
-      sa.load(a, m0, k0 + BK, M, ke);
-      sb.load(b, n0, k0 + BK, N, ke);
+  for (int half = 0; half < HALVES; ++half) {
+    const Operand now{half ? a.rest : a.p, a.ld, a.whole, a.words, nullptr};
+    if (kb < ke) {
+      sa.load(now, m0, kb, M, ke);
+      sb.load(b, n0, kb, N, ke);
     }
-    if constexpr (sizeof(T) == 2) {
-      b8 fa[FM], fb[FN];
+    for (int64_t k0 = kb; k0 < ke; k0 += BK) {
+      sa.store(as);
+      sb.store(bs);
+      __syncthreads();
+      if (k0 + BK < ke) {
+        sa.load(now, m0, k0 + BK, M, ke);
+        sb.load(b, n0, k0 + BK, N, ke);
+      }
+      if constexpr (sizeof(T) == 2) {
+        b8 fa[FM], fb[FN];
 #pragma unroll
-      for (int i = 0; i < FM; ++i)
-        fa[i] = *(const b8*)(as + (wm + i * 16 + (lane & 15)) * LD + (lane >> 4) * 8);
-#pragma unroll
-      for (int j = 0; j < FN; ++j)
-        fb[j] = *(const b8*)(bs + (wn + j * 16 + (lane & 15)) * LD + (lane >> 4) * 8);
-#pragma unroll
-      for (int i = 0; i < FM; ++i)
+        for (int i = 0; i < FM; ++i)
+          fa[i] = *(const b8*)(as + (wm + i * 16 + (lane & 15)) * LD + (lane >> 4) * 8);
 #pragma unroll
         for (int j = 0; j < FN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i], fb[j], acc[i][j], 0, 0, 0);
-    } else {
-#pragma unroll
-      for (int s = 0; s < BK; s += 4) {
-        float fa[FM], fb[FN];
-#pragma unroll
-        for (int i = 0; i < FM; ++i) fa[i] = as[(wm + i * 16 + (lane & 15)) * LD + s + (lane >> 4)];
-#pragma unroll
-        for (int j = 0; j < FN; ++j) fb[j] = bs[(wn + j * 16 + (lane & 15)) * LD + s + (lane >> 4)];
+          fb[j] = *(const b8*)(bs + (wn + j * 16 + (lane & 15)) * LD + (lane >> 4) * 8);
 #pragma unroll
         for (int i = 0; i < FM; ++i)
 #pragma unroll
           for (int j = 0; j < FN; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fa[i], fb[j], acc[i][j], 0, 0, 0);
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i], fb[j], acc[i][j], 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int s = 0; s < BK; s += 4) {
+          float fa[FM], fb[FN];
+#pragma unroll
+          for (int i = 0; i < FM; ++i) fa[i] = as[(wm + i * 16 + (lane & 15)) * LD + s + (lane >> 4)];
+#pragma unroll
+          for (int j = 0; j < FN; ++j) fb[j] = bs[(wn + j * 16 + (lane & 15)) * LD + s + (lane >> 4)];
+#pragma unroll
+          for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fa[i], fb[j], acc[i][j], 0, 0, 0);
+        }
       }
+      __syncthreads();
     }
-    __syncthreads();
   }
 #pragma unroll
   for (int i = 0; i < FM; ++i)
@@ -339,9 +344,9 @@ struct Direct {
     base += step;
   }
 #pragma clang diagnostic pop
-  // the `left` values of k behind `steps` whole tiles
-  __device__ __forceinline__ void load_tail(T* lds, int64_t steps, int left) const {
-    const T* p = base + steps * step;
+  // the `left` values of k behind `steps` whole tiles, `away` from here
+  __device__ __forceinline__ void load_tail(T* lds, int64_t steps, int left, int64_t away = 0) const {
+    const T* p = base + away + steps * step;
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       int r, k;
@@ -405,7 +410,8 @@ __device__ __forceinline__ void tile_of(int64_t b, int64_t rows, int64_t cols, i
   c = t % band / height;
 }
 
-template <typename T, bool AX, bool BX, int ACT, int BM, int BN, int WM, int WN, int LB>
+// HALVES as in gemm_kernel. (A kernel for both takes up to 5% longer where there is one.)
+template <typename T, bool AX, bool BX, int ACT, int BM, int BN, int WM, int WN, int LB, int HALVES>
 __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_large_kernel(
     Operand a, Operand b, int64_t M, int64_t N, int64_t Kd, int64_t a_end, int64_t b_end, int64_t k_part,
     int64_t row_tiles, int64_t col_tiles, Epilogue e, float* __restrict__ ws) {
@@ -424,7 +430,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_large_kernel(
   const int64_t m0 = tr * BM, n0 = tc * BN;
   const int64_t kb = blockIdx.y * k_part, ke = min(Kd, kb + k_part);
   const int tiles = (int)((max(ke, kb) - kb) / FK), left = (int)((max(ke, kb) - kb) % FK);
-  const int steps = tiles + (left > 0);
+  const int64_t away = HALVES == 2 ? (const T*)a.rest - (const T*)a.p : 0;
+  const int lead = left > 0 ? HALVES : 0;  // what is left over of k comes first, of both halves
+  const int steps = HALVES * tiles + lead;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
   A du, dl;
@@ -432,13 +440,20 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_large_kernel(
   du.init(a, m0, kb, a_end);
   dl.init(a, m0 + H * 16, kb, a_end);
   db.init(b, n0, kb, b_end);
-  // what is left over of k comes first
-  if (left > 0) {
-    du.load_tail(up(0), tiles, left);
-    dl.load_tail(low(0), tiles, left);
-    db.load_tail(bs(0), tiles, left);
+  for (int s = 0; s < lead; ++s) {
+    du.load_tail(up(s), tiles, left, s * away);
+    dl.load_tail(low(s), tiles, left, s * away);
+    db.load_tail(bs(s), tiles, left);
   }
-  for (int s = left > 0; s < min(steps, 2); ++s) {
+  // before step s is loaded: whether it is the second half's first, for which B starts again
+  const auto turn = [&](int s) {
+    if (HALVES == 1 || s != lead + tiles) return;
+    du.base += away - tiles * du.step;
+    dl.base += away - tiles * dl.step;
+    db.base -= tiles * db.step;
+  };
+  for (int s = lead; s < min(steps, 2); ++s) {
+    turn(s);
     du.load(up(s), wave);
     db.load(bs(s), wave);
     dl.load(low(s), wave);
@@ -491,6 +506,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_large_kernel(
     barrier(!more);
     read_a(a0, low(at), 0);
     if (more) {
+      turn(s + 2);
       du.load(up(at), wave);
       db.load(bs(at), wave);
     }
@@ -596,15 +612,26 @@ __global__ __launch_bounds__(NT) void join_kernel(const float* __restrict__ ws, 
 // gradient). 64 columns a block, a wave a row. A relu's z is told by y = relu(z) as well: they are above zero together.
 // dz is rounded to the operands' type, which the matrix instructions of dx and dW take; its sum is of
 // what it was before. In bf16 that is half a step a value, and with silu or gelu, whose dz is no copy
-// of dy, dx and dW are 1.44 times as far from their formula as with dz in fp32 (2.4e-3 against 1.7e-3,
-// relative; 1.0 to 2.2 times where they have some dozen values), nearly all of it by dz, not by z.
-// Both halves of dz through the products would keep it, at twice their time.
+// of dy, dx and dW would be 1.44 times as far from their formula as with dz in fp32 (2.4e-3 against
+// 1.7e-3, relative; 1.0 to 2.2 times where they have some dozen values). What it is rounded by goes to
+// `rest`, in bf16 too, and through the products beside it: 16 bits of dz are kept. All of a pass with
+// gradients takes 1.1 times as long for it at 64x3136x2048 (37 us, 41), 1.5 at 2048x2048x2048 (89, 132)
+// and 1.56 at 8192x4096x12288 (2.04 ms, 3.18).
+template <typename T, int ACT>
+constexpr bool HAS_REST = sizeof(T) == 2 && ACT >= ACT_SILU;
+template <typename T>
+__device__ __forceinline__ float rest_of(float d) {  // of what is not finite there is none
+  const float kept = to_float(from_float<T>(d));
+  return fabsf(kept) < __builtin_inff() ? d - kept : 0.f;
+}
+
 template <typename T, int ACT>
 __global__ __launch_bounds__(NT) void act_bwd_kernel(const T* __restrict__ dy,
                                                      const T* __restrict__ z, int64_t M, int64_t N,
                                                      int64_t col_tiles, int64_t chunk,
-                                                     T* __restrict__ dz, float* __restrict__ ws,
-                                                     void* __restrict__ db, bool is_float) {
+                                                     T* __restrict__ dz, T* __restrict__ rest, int64_t ld,
+                                                     float* __restrict__ ws, void* __restrict__ db,
+                                                     bool is_float) {
   __shared__ float part[NT / 64][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t c = blockIdx.x % col_tiles * 64 + lane, k = blockIdx.x / col_tiles;
@@ -616,7 +643,9 @@ __global__ __launch_bounds__(NT) void act_bwd_kernel(const T* __restrict__ dy,
       float d = to_float(dy[at]);
       if constexpr (ACT != ACT_NONE) {
         d = act_bwd<T, ACT>(d, to_float(z[at]));
-        dz[at] = from_float<T>(d);
+        dz[r * ld + c] = from_float<T>(d);
+        if constexpr (HAS_REST<T, ACT>)
+          if (rest) rest[r * ld + c] = from_float<T>(rest_of<T>(d));
       }
       s += d;
     }
@@ -639,7 +668,8 @@ template <typename T, int ACT>
 __global__ __launch_bounds__(NT) void act_bwd_vector_kernel(const T* __restrict__ dy,
                                                             const T* __restrict__ z, int64_t M,
                                                             int64_t N, int64_t col_tiles, int64_t chunk,
-                                                            T* __restrict__ dz, float* __restrict__ ws,
+                                                            T* __restrict__ dz, T* __restrict__ rest,
+                                                            int64_t ld, float* __restrict__ ws,
                                                             void* __restrict__ db, bool is_float) {
   constexpr int V = 16 / sizeof(T), WIDE = 32 * V, AHEAD = 4;
   __shared__ float part[8][WIDE];
@@ -668,7 +698,14 @@ __global__ __launch_bounds__(NT) void act_bwd_vector_kernel(const T* __restrict_
           if constexpr (ACT != ACT_NONE) {
 #pragma unroll
             for (int v = 0; v < V / 2; ++v) d[i].set2(v, g[2 * v], g[2 * v + 1]);
-            d[i].store(dz + (r + 8 * i) * N + c);
+            d[i].store(dz + (r + 8 * i) * ld + c);
+            if constexpr (HAS_REST<T, ACT>)
+              if (rest) {
+#pragma unroll
+                for (int v = 0; v < V / 2; ++v)
+                  d[i].set2(v, rest_of<T>(g[2 * v]), rest_of<T>(g[2 * v + 1]));
+                d[i].store(rest + (r + 8 * i) * ld + c);
+              }
           }
         }
     }
@@ -711,7 +748,7 @@ const void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; 
 Operand operand(const Tensor& t) {
   const int64_t size = t.element_size(), ld = t.size(0) > 1 ? t.stride(0) : 0;
   const uintptr_t at = (uintptr_t)t.data_ptr();
-  return {t.data_ptr(), ld, ld * size % 16 == 0 && at % 16 == 0, ld * size % 4 == 0 && at % 4 == 0};
+  return {t.data_ptr(), ld, ld * size % 16 == 0 && at % 16 == 0, ld * size % 4 == 0 && at % 4 == 0, nullptr};
 }
 
 bool rows_of_8(int64_t N, std::initializer_list<const void*> ptrs) {
@@ -767,11 +804,12 @@ constexpr TileShape TILES[] = {
 // on. bf16, M x K x N: 2048x12288x4096 takes 278 us in tiles of 256x256 and 205 in two parts, 184 in
 // 256x128, 198 in 128x128; 1024x1024x1024 14 in 128x128, 9 in 64x64; 64x3136x2048 19 in 64x64 whole,
 // 8.5 in 8 parts; 1x4096x12288 39 whole, 19 in 2 parts, 22 in 8.
-Choice choose(int64_t M, int64_t N, int64_t Kd, int64_t elem, bool by_words) {
+// `halves`: 2 where A comes in two, and the sum is gone over twice.
+Choice choose(int64_t M, int64_t N, int64_t Kd, int64_t elem, bool by_words, int halves) {
   Choice best{0, 1};
   double least = 1e30;
   const int64_t steps = ceil_div(Kd * elem, ROW_BYTES);
-  const double bytes = (double)(M * Kd + N * Kd + M * N) * elem;
+  const double bytes = (double)(halves * M * Kd + N * Kd + M * N) * elem;
   for (int t = by_words ? 2 : 0; t < 4; ++t) {
     const TileShape& s = TILES[t];
     const int64_t tiles = ceil_div(M, s.bm) * ceil_div(N, s.bn);
@@ -779,7 +817,7 @@ Choice choose(int64_t M, int64_t N, int64_t Kd, int64_t elem, bool by_words) {
          parts *= 2) {
       const int64_t a_cu = ceil_div(tiles * parts, 256), full = a_cu / s.per_cu, rest = a_cu % s.per_cu;
       const double* us = elem == 2 ? s.bf16_us : s.fp32_us;
-      const double part = (double)ceil_div(steps, parts);
+      const double part = (double)(halves * ceil_div(steps, parts));
       const double last = 2 + 1.5e-4 * s.bm * s.bn * s.per_cu;  // and the tile's way out
       double cost = full * (part * us[s.per_cu - 1] + last) + (rest ? part * us[rest - 1] + last : 0);
       cost = std::max(cost, bytes / 5e6 * std::max(1.0, 256.0 / (tiles * parts)));
@@ -793,14 +831,24 @@ Choice choose(int64_t M, int64_t N, int64_t Kd, int64_t elem, bool by_words) {
   return best;
 }
 
+// only going back, in bf16, does A come in two halves
+template <typename T, bool BX>
+constexpr bool MAY_HALVE = BX && sizeof(T) == 2;
+
 template <typename T, bool AX, bool BX, int ACT, int BM, int BN, int WM, int WN, int LB = 16>
 void launch_large(const Operand& a, const Operand& b, int64_t M, int64_t N, int64_t Kd, int64_t Ma,
                   int64_t Nb, int64_t parts, const Epilogue& e, float* ws, hipStream_t st) {
   const int64_t rows = ceil_div(M, BM), cols = ceil_div(N, BN), values = ROW_BYTES / sizeof(T);
   const int64_t part = ceil_div(ceil_div(Kd, parts), values) * values;
-  gemm_large_kernel<T, AX, BX, ACT, BM, BN, WM, WN, LB>
-      <<<dim3(grid_of(rows * cols, 64 * WM * WN, "linear_act"), (unsigned)parts), 64 * WM * WN, 0, st>>>(
-          a, b, M, N, Kd, Ma, Nb, part, rows, cols, e, ws);
+  const dim3 grid(grid_of(rows * cols, 64 * WM * WN, "linear_act"), (unsigned)parts);
+  if constexpr (MAY_HALVE<T, BX>)
+    if (a.rest) {
+      gemm_large_kernel<T, AX, BX, ACT, BM, BN, WM, WN, LB, 2>
+          <<<grid, 64 * WM * WN, 0, st>>>(a, b, M, N, Kd, Ma, Nb, part, rows, cols, e, ws);
+      return;
+    }
+  gemm_large_kernel<T, AX, BX, ACT, BM, BN, WM, WN, LB, 1>
+      <<<grid, 64 * WM * WN, 0, st>>>(a, b, M, N, Kd, Ma, Nb, part, rows, cols, e, ws);
 }
 
 template <typename T, bool AX, bool BX, int ACT>
@@ -808,9 +856,13 @@ void launch_small(const Operand& a, const Operand& b, int64_t M, int64_t N, int6
                   const Epilogue& e, float* ws, hipStream_t st) {
   const int64_t rows = ceil_div(M, 64), cols = ceil_div(N, 64);
   const int64_t part = ceil_div(ceil_div(Kd, parts), Tile<T>::BK) * Tile<T>::BK;
-  gemm_kernel<T, AX, BX, ACT, 64, 64>
-      <<<dim3(grid_of(rows * cols, NT, "linear_act"), (unsigned)parts), NT, 0, st>>>(a, b, M, N, Kd, part,
-                                                                                  cols, e, ws);
+  const dim3 grid(grid_of(rows * cols, NT, "linear_act"), (unsigned)parts);
+  if constexpr (MAY_HALVE<T, BX>)
+    if (a.rest) {
+      gemm_kernel<T, AX, BX, ACT, 64, 64, 2><<<grid, NT, 0, st>>>(a, b, M, N, Kd, part, cols, e, ws);
+      return;
+    }
+  gemm_kernel<T, AX, BX, ACT, 64, 64, 1><<<grid, NT, 0, st>>>(a, b, M, N, Kd, part, cols, e, ws);
 }
 
 // Rows off the 16 bytes. Where they lie on 4, as fp32 always does, lanes load 4 bytes each: fp32
@@ -822,23 +874,26 @@ void launch_small(const Operand& a, const Operand& b, int64_t M, int64_t N, int6
 // and 198.
 constexpr double PAD_WORDS = 8e9, PAD_ODD = 8e8;
 
-// out [M, N] = A B^T over Kd, A and B with k along (or across) their rows in memory
+// out [M, N] = A B^T over Kd, A and B with k along (or across) their rows in memory; A plus `rest`,
+// where there is one, and then A's rows are whole vectors
 template <bool AX, bool BX>
 void gemm(const Tensor& a, const Tensor& b, int64_t M, int64_t N, int64_t Kd, const Epilogue& e,
-          const Tensor& like) {
+          const Tensor& like, const Tensor& rest = Tensor()) {
   if (M == 0 || N == 0) return;
   const hipStream_t st = stream_of(like);
   Operand oa = operand(a), ob = operand(b);
+  oa.rest = ptr(rest);
+  const int halves = oa.rest ? 2 : 1;
   const int64_t elem = like.element_size(), E = 16 / elem;
+  int64_t Ma = AX && oa.rest ? ceil_div(M, E) * E : M, Nb = N;  // rows that may be read
   // offsets within a tile are 32 bits
   bool large = Kd > 0 && std::max(oa.ld, ob.ld) * 256 * elem < (1LL << 32);
-  const bool fits_a = oa.whole && (!AX || M % E == 0), fits_b = ob.whole && (!BX || N % E == 0);
-  const bool words = oa.words && ob.words && (!AX || M * elem % 4 == 0) && (!BX || N * elem % 4 == 0);
-  int64_t Ma = M, Nb = N;  // rows that may be read
+  const bool fits_a = oa.whole && (!AX || Ma % E == 0), fits_b = ob.whole && (!BX || N % E == 0);
+  const bool words = oa.words && ob.words && (!AX || Ma * elem % 4 == 0) && (!BX || N * elem % 4 == 0);
   bool by_words = false;
   Tensor padded;
   if (large && !(fits_a && fits_b)) {
-    const double work = (double)M * N * Kd;
+    const double work = (double)M * N * Kd * halves;
     by_words = words && (elem == 4 || work < PAD_WORDS);
     large = by_words || work >= PAD_ODD;
     if (large && !by_words) {
@@ -856,14 +911,14 @@ void gemm(const Tensor& a, const Tensor& b, int64_t M, int64_t N, int64_t Kd, co
       // a block a row, as far as a launch has blocks
       const unsigned rows = (unsigned)std::min<int64_t>(pa.rows + pb.rows, 1 << 20);
       MM_DISPATCH_TYPE(like, (pad_kernel<T><<<rows, NT, 0, st>>>(pa, pb)));
-      if (!fits_a) oa = {pa.to, pa.ld, true, true}, Ma = AX ? pa.ld : M;
-      if (!fits_b) ob = {pb.to, pb.ld, true, true}, Nb = BX ? pb.ld : N;
+      if (!fits_a) oa = {pa.to, pa.ld, true, true, nullptr}, Ma = AX ? pa.ld : M;
+      if (!fits_b) ob = {pb.to, pb.ld, true, true, nullptr}, Nb = BX ? pb.ld : N;
       if (!fits_a && !fits_b) Kd = ceil_div(Kd, step) * step;
     }
   }
   Choice c{0, 1};
   if (large) {
-    c = choose(M, N, Kd, elem, by_words);
+    c = choose(M, N, Kd, elem, by_words, halves);
   } else {
     // few tiles: the sum is split over k, 128 values a part at least
     c.parts = std::max<int64_t>(1, std::min(ceil_div(512, ceil_div(M, 64) * ceil_div(N, 64)), Kd / 128));
@@ -966,7 +1021,11 @@ class LinearAct : public torch::autograd::Function<LinearAct> {
     int64_t M = 1;
     for (size_t i = 0; i + 1 < sizes.size(); ++i) M *= sizes[i];
     const hipStream_t st = stream_of(dy);
-    Tensor dz = act == ACT_NONE ? dy : at::empty_like(dy), db;
+    // [M, N]; in two halves its rows are filled up to whole vectors, with what nobody reads
+    const bool halves = act >= ACT_SILU && dy.scalar_type() == at::kBFloat16 && (needs & 3);
+    const int64_t ld = halves ? ceil_div(N, 8) * 8 : N;
+    Tensor dz = act == ACT_NONE ? dy.view({M, N}) : at::empty({M, ld}, dy.options()).narrow(1, 0, N), db;
+    const Tensor rest = halves ? at::empty({M, ld}, dy.options()) : Tensor();
     const bool need_b = needs & 4;
     if (need_b)
       db = at::empty({N}, dy.options().dtype(ctx->saved_data["bias_float"].toBool() ? at::kFloat
@@ -975,7 +1034,8 @@ class LinearAct : public torch::autograd::Function<LinearAct> {
       if (need_b) db.zero_();
     } else if (need_b || act != ACT_NONE) {
       const bool vectors = N * dy.element_size() % 16 == 0 && (uintptr_t)dy.data_ptr() % 16 == 0 &&
-                           (uintptr_t)dz.data_ptr() % 16 == 0 && (uintptr_t)ptr(saved[2]) % 16 == 0;
+                           (uintptr_t)dz.data_ptr() % 16 == 0 && (uintptr_t)ptr(rest) % 16 == 0 &&
+                           (uintptr_t)ptr(saved[2]) % 16 == 0;
       const int64_t cols = ceil_div(N, vectors ? 512 / dy.element_size() : 64);
       // up to 128 rows one chunk, which needs no second launch; else as many as fill the CUs, and
       // 256 at most, which 16 waves join in 16 steps
@@ -990,26 +1050,25 @@ class LinearAct : public torch::autograd::Function<LinearAct> {
       MM_DISPATCH_TYPE(dy, MM_DISPATCH_ACT(act, {
         const auto kernel = vectors ? &act_bwd_vector_kernel<T, ACT> : &act_bwd_kernel<T, ACT>;
         kernel<<<grid_of(cols * chunks, NT, "linear_act"), NT, 0, st>>>(
-            (const T*)ptr(dy), (const T*)ptr(saved[2]), M, N, cols, chunk, (T*)dz.data_ptr(), wp,
-            once, bias_float);
+            (const T*)ptr(dy), (const T*)ptr(saved[2]), M, N, cols, chunk, (T*)dz.data_ptr(),
+            (T*)ptr(rest), ld, wp, once, bias_float);
       }));
       if (wp)
         bias_grad_kernel<<<grid_of(ceil_div(N, 64), 1024, "linear_act"), 1024, 0, st>>>(wp, chunks, N, bias_float, db.data_ptr());
       check_launch("linear_act backward");
     }
-    const Tensor dzm = dz.view({M, N});
     Tensor dx, dw;
     if (needs & 1) {
       dx = at::empty(sizes, dy.options());
       Epilogue e{nullptr, false, nullptr, nullptr, dx.data_ptr(), ACT_NONE, rows_of_8(Kd, {ptr(dx)})};
-      gemm<false, true>(dzm, saved[1], M, Kd, N, e, dy);
+      gemm<false, true>(dz, saved[1], M, Kd, N, e, dy, rest);
     }
     if (needs & 2) {
       dw = at::empty({N, Kd}, dy.options());
       Epilogue e{nullptr, false, nullptr, nullptr, dw.data_ptr(), ACT_NONE, rows_of_8(Kd, {ptr(dw)})};
-      gemm<true, true>(dzm, saved[0].dim() == 2 ? saved[0] : saved[0].reshape({M, Kd}), N, Kd, M, e, dy);
+      gemm<true, true>(dz, saved[0].dim() == 2 ? saved[0] : saved[0].reshape({M, Kd}), N, Kd, M, e, dy, rest);
     }
-    return {dx, dw, db, needs & 8 ? dz : Tensor(), Tensor()};
+    return {dx, dw, db, needs & 8 ? dz.view(dy.sizes()) : Tensor(), Tensor()};
   }
 };
 

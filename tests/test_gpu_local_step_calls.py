@@ -228,3 +228,47 @@ def test_activations_in_fp32_hold_its_bits():
                 U * ((2 * d * d + 12) * cdf + d.abs() * pdf * (d * d + 8))[near])
         assert torch.equal(y.detach().view(-1)[z.cuda() > 9], z.cuda()[z.cuda() > 9])
         assert y.detach().view(-1)[z.cuda() < -9].abs().max() < 1e-17
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("m,k,n", [
+    (96, 64, 128), (65, 33, 71), (1, 8, 24), (300, 130, 66), (512, 512, 512), (1000, 1001, 999),
+    (1030, 1024, 1018), (700, 4096, 1024), (4096, 256, 40),
+])
+def test_linear_keeps_the_activations_gradient(m, k, n, act):
+    """Each row of x picks a row of W^T, so z is a value of W and exact in bf16, and of dx and dW
+    there is left: dz in fp32 (the activation's derivative within 2^-20), its rest behind two halves
+    of 8 bits, 2^-16, the products' sums, and one rounding to bf16."""
+    half = torch.finfo(BF16).eps / 2
+    pick = torch.randint(0, k, (m,), generator=torch.Generator().manual_seed(m + n))
+    x = torch.nn.functional.one_hot(pick, k).to(BF16)
+    w, dy = _randn((n, k), BF16, 1), _randn((m, n), BF16, 2)
+    b = torch.zeros(n)
+    z = (x.double() @ w.double().t()).requires_grad_(True)
+    dz, = torch.autograd.grad(getattr(torch.nn.functional, act)(z), z, dy.double())
+    leaves = [t.cuda().requires_grad_(True) for t in (x, w, b)]
+    dx, dw, db = torch.autograd.grad(ops.linear_act(*leaves, act=act), leaves, dy.cuda())
+    edz = 2.0 ** -20 * dy.double().abs()
+    kept = edz + 2.0 ** -16 * (dz.abs() + edz)
+    want, mag = dz @ w.double(), dz.abs() @ w.double().abs()
+    tol = kept @ w.double().abs() + (2 * n + 8) * U * mag
+    _within(dx, want, tol + half * (want.abs() + tol))
+    want, mag = dz.t() @ x.double(), dz.abs().t() @ x.double()
+    tol = kept.t() @ x.double() + (2 * m + 8) * U * mag
+    _within(dw, want, tol + half * (want.abs() + tol))
+    _within(db, dz.sum(0), (edz + (m + 8) * U * dz.abs()).sum(0))
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_linear_gradients_that_are_not_finite_stay_in_their_row(act):
+    x, w, dy = _randn((70, 40), BF16, 1).cuda(), _randn((48, 40), BF16, 2).cuda(), _randn((70, 48), BF16, 3).cuda()
+    x, w = x.requires_grad_(True), w.requires_grad_(True)
+    y = ops.linear_act(x, w, act=act)
+    want, = torch.autograd.grad(y, x, dy, retain_graph=True)
+    # the last of bf16's values: its dz is infinite, or is rounded to infinity, or neither
+    dy[4, 7], dy[9, 3], dy[11] = math.inf, math.nan, torch.finfo(BF16).max
+    dx, = torch.autograd.grad(y, x, dy)
+    odd = torch.zeros(70, dtype=torch.bool, device="cuda")
+    odd[[4, 9, 11]] = True
+    assert torch.equal(dx[~odd], want[~odd])
+    assert not torch.isfinite(dx[4]).any() and torch.isnan(dx[9]).all()
