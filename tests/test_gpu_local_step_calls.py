@@ -272,3 +272,113 @@ def test_linear_gradients_that_are_not_finite_stay_in_their_row(act):
     odd[[4, 9, 11]] = True
     assert torch.equal(dx[~odd], want[~odd])
     assert not torch.isfinite(dx[4]).any() and torch.isnan(dx[9]).all()
+
+
+def _plain_loss(params, x, target):
+    """A pixel-wise linear, group norm with relu, a linear with residual and silu."""
+    f = torch.nn.functional
+    h = f.linear(x, params[0]).permute(0, 3, 1, 2)
+    h = torch.relu(f.group_norm(h.contiguous(), 2, params[1], params[2])).permute(0, 2, 3, 1)
+    y = f.silu(f.linear(h.reshape(12, 72), params[3], params[4]) + target)
+    return (y - 1).square().mean()
+
+
+def test_a_step_goes_against_its_gradient():
+    """The three operators together against the same step in 64 bits. AdamW's first step moves each
+    parameter by lr against its gradient's sign; that is certain where a gradient is over a quarter of
+    its tensor's largest: 64 roundings of bf16, 2^-8 each, all one way, would be needed to turn it."""
+    sizes = [(8, 16), (8,), (8,), (40, 72), (40,)]
+    flat = torch.cat([_randn((math.prod(s),), FP32, i) * (0.1 if i != 2 else 1) + (i == 1)
+                      for i, s in enumerate(sizes)]).to(BF16)
+    x, target = _randn((12, 3, 3, 16), BF16, 7), _randn((12, 40), BF16, 8)
+    wide = [p.view(s).double().requires_grad_(True) for p, s in zip(flat.split([math.prod(s) for s in sizes]), sizes)]
+    loss = _plain_loss(wide, x.double(), target.double())
+    grads = torch.autograd.grad(loss, wide)
+
+    dev = flat.cuda()
+    state = ops.adamw_state(dev.numel(), "cuda", 8)
+    params = [p.view(s).detach().requires_grad_(True) for p, s in zip(dev.split([math.prod(s) for s in sizes]), sizes)]
+    h = ops.linear_act(x.cuda(), params[0]).permute(0, 3, 1, 2)
+    h = ops.group_norm_act(h, 2, params[1], params[2], act="relu").permute(0, 2, 3, 1)
+    y = ops.linear_act(h.reshape(12, 72), params[3], params[4], act="silu", res=target.cuda())
+    got = (y.float() - 1).square().mean()
+    # y is within some roundings of bf16 of its values, which lie below 8
+    assert abs(got.item() - loss.item()) <= 8 * 8 * 2.0 ** -8 * loss.sqrt().item()
+    ops.adamw_step([p.detach() for p in params], torch.autograd.grad(got, params), *state, 2.0 ** -6,
+                   weight_decay=0.0, seed=4)
+    m = ops.adamw_dequantize(*state[:2])[0].cpu().split([math.prod(s) for s in sizes])
+    for p, q, g, first in zip(wide, params, grads, m):
+        sure = g.abs() > 0.25 * g.abs().max()
+        assert sure.any()
+        want = (p - 2.0 ** -6 * g.sign())[sure]
+        # a step of bf16 for its rounding, and what the moments' eps leaves of lr
+        _within(q.detach()[sure.cuda()], want.detach(), 2.0 ** -7 * want.detach().abs() + 1e-4 * 2.0 ** -6)
+        assert (first.view(g.shape)[sure].sign() == g[sure].sign()).all()
+
+
+def test_captured_and_eager_epochs_agree_where_gradients_are_large(monkeypatch):
+    """16 samples summed in another order change a gradient by 16 * 24 u of what enters its sum.
+    Where a first moment is over a tenth of its largest, that is at most 64 times the gradient, and
+    a step changes by twice that share of lr; four steps."""
+    from torch.utils.data import DataLoader, TensorDataset
+
+    from murmura_amd.aggregation.fedavg import FedAvgAggregator
+    from murmura_amd.core.node import Node
+    from murmura_amd.core.optim import AdamWConfig
+    from murmura_amd.models import SimpleMLP
+
+    def train(graphs):
+        if not graphs:
+            monkeypatch.setenv("MURMURA_NO_GRAPHS", "1")
+        torch.manual_seed(0)
+        data = TensorDataset(_randn((16, 24), FP32, 9), torch.arange(16) % 4)
+        loader = DataLoader(data, batch_size=16)
+        node = Node(0, SimpleMLP(24, 64, 4, fused=True), loader, loader, FedAvgAggregator(),
+                    torch.device("cuda"), dtype=FP32, optimizer=AdamWConfig())
+        for _ in range(4):
+            node.local_train(lr=1e-2)
+        monkeypatch.delenv("MURMURA_NO_GRAPHS", raising=False)
+        return node
+
+    a, b = train(True), train(False)
+    sure = a.optimizer.exp_avg.abs() > 0.1 * a.optimizer.exp_avg.abs().max()
+    assert sure.sum() > 20
+    assert (a.get_state() - b.get_state())[sure].abs().max() <= 4 * 2 * 1e-2 * 16 * 24 * U * 64
+
+
+@pytest.mark.parametrize("n,c,h,groups,act", [(128, 256, 56, 32, "silu"), (37, 48, 61, 3, "gelu"), (2, 64, 200, 8, "relu")])
+def test_group_norm_repeats_between_other_calls(n, c, h, groups, act):
+    """The same bits each time, in whichever of the three forms: held, read twice, by chunks."""
+    def state(seed):
+        g = torch.Generator("cuda").manual_seed(seed)
+        images = [torch.randn(n, h, h, c, generator=g, device="cuda").to(BF16).permute(0, 3, 1, 2) for _ in range(2)]
+        w, b = (torch.randn(c, generator=g, device="cuda").to(BF16) for _ in range(2))
+        return [t.requires_grad_(True) for t in (images[0], w, b)], images[1]
+
+    def run(leaves, dy):
+        y = ops.group_norm_act(leaves[0], groups, leaves[1], leaves[2], act=act)
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    one, two = state(1), state(2)
+    first = run(*one)
+    for _ in range(3):
+        run(*two)
+        assert all(torch.equal(p, q) for p, q in zip(first, run(*one)))
+
+
+@pytest.mark.parametrize("act", ["relu", "silu"])
+def test_linear_repeats_between_other_calls(act):
+    """Sums split over parts are joined in their order."""
+    def run(seed, m, k, n):
+        g = torch.Generator("cuda").manual_seed(seed)
+        x, w, dy = (torch.randn(s, generator=g, device="cuda").to(BF16) for s in ((m, k), (n, k), (m, n)))
+        b = torch.randn(n, generator=g, device="cuda")
+        leaves = [t.requires_grad_(True) for t in (x, w, b)]
+        y = ops.linear_act(*leaves, act=act)
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    for sizes in ((64, 3136, 2048), (1000, 1001, 999), (2048, 2048, 2048), (5, 7000, 40)):
+        first = run(1, *sizes)
+        for _ in range(3):
+            run(2, *sizes)
+            assert all(torch.equal(p, q) for p, q in zip(first, run(1, *sizes)))
