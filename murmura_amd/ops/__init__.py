@@ -222,10 +222,12 @@ def scale_inject(flat: Tensor, lam: float) -> Tensor:
 
 
 # ------------------------------------------------- under torch.vmap (K16, K18)
+_transforms_active = torch._C._are_functorch_transforms_active
+
+
 def _is_mapped(*tensors: Optional[Tensor]) -> bool:
-    """Whether torch.vmap is at work on one of them: those have no memory that a kernel could read."""
-    if not torch._C._are_functorch_transforms_active():
-        return False
+    """Whether torch.vmap, where a transform is active, is at work on one of them: those have no
+    memory that a kernel could read."""
     functorch = torch._C._functorch
     return functorch.peek_interpreter_stack().key() == functorch.TransformType.Vmap and any(
         t is not None and functorch.is_batchedtensor(t) for t in tensors)
@@ -282,7 +284,7 @@ def group_norm_act(x: Tensor, num_groups: int, weight: Optional[Tensor] = None,
     call; other transforms, and a derivative going forward, are refused on a GPU."""
     ref.check_group_norm_act(x, num_groups, weight, bias, res)
     code = ref.check_act(act)
-    if _is_mapped(x, weight, bias, res):
+    if _transforms_active() and _is_mapped(x, weight, bias, res):
         return _MappedGroupNormAct.apply(x, num_groups, weight, bias, eps, act, res)
     if _use_native(x):
         return _EXT.group_norm_act(x, num_groups, weight, bias, eps, code, res)
@@ -363,7 +365,7 @@ def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: st
     ref.check_linear_act(x, weight, bias, res)
     code = ref.check_act(act)
     if _use_native(x):
-        if _is_mapped(x, weight, bias, res):
+        if _transforms_active() and _is_mapped(x, weight, bias, res):
             return _MappedLinearAct.apply(x, weight, bias, act, res)
         return _EXT.linear_act(x, weight, bias, code, res)
     return ref.linear_act(x, weight, bias, act, res)
