@@ -501,7 +501,8 @@ void adamw_step(const std::vector<Tensor>& params, std::vector<Tensor> grads,
       t.s[t.count++] = {params[i].data_ptr(), grads[i].data_ptr(), at};
       at += params[i].numel();
     }
-    t.end = i == params.size() ? P : eight ? at / QB * QB : at;
+    const int64_t unit = eight ? QB : 8;  // and a launch starts on whole vectors of the moments
+    t.end = i == params.size() ? P : at / unit * unit;
     t.last = t.end == P;
     while (next < i && start + params[next].numel() <= t.end) start += params[next++].numel();
     return t;
