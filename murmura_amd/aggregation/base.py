@@ -20,6 +20,7 @@ import torch
 from torch import Tensor
 
 from murmura_amd import ops
+from murmura_amd.ops.fused_norm import MurmuraGroupNorm
 
 
 class EvalContext:
@@ -40,7 +41,7 @@ class EvalContext:
         # in one pass, 7.4 one by one; FEMNIST's two convolutions 0.5 and 1.2. (With
         # batch norm it goes one by one as well: its kernels know no vmap.)
         if torch.device(device).type == "cuda" and any(
-                isinstance(m, torch.nn.GroupNorm) for m in store.model.modules()):
+                isinstance(m, MurmuraGroupNorm) for m in store.model.modules()):
             self._vmap_ok = False
 
     _device_batches: "list | None" = None
