@@ -979,7 +979,8 @@ Forward forward_of(const Tensor& x, const Tensor& weight, const Tensor& bias, co
   const Tensor res = residual.defined() ? residual.contiguous() : residual;
   f.y = at::empty(sizes, x.options());
   // silu and gelu have to see z again. It is kept in the operands' type, as a layer that writes
-  // it out would keep it.
+  // it out would keep it: in bf16, dx, dW and db are 1.06 times as far from their formula as with z in
+  // fp32 (1.0 to 1.3 times where they have some dozen values), for half of its memory.
   const bool keep_z = differentiable && (act == ACT_SILU || act == ACT_GELU);
   if (keep_z) f.keep = at::empty(sizes, x.options());
   Epilogue e{ptr(b), b.defined() && b.scalar_type() == at::kFloat, ptr(res), (void*)ptr(f.keep),
