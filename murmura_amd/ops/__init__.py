@@ -345,6 +345,9 @@ def adamw_dequantize(exp_avg: ref.Moment, exp_avg_sq: ref.Moment,
     """The values of 8-bit moments, in fp32 or bf16 (which holds them as they are)."""
     if dtype not in (torch.float32, torch.bfloat16):
         raise ValueError(f"adamw_dequantize: fp32 or bf16, not {dtype}")
+    if isinstance(exp_avg, Tensor) or isinstance(exp_avg_sq, Tensor):
+        raise ValueError("adamw_dequantize: moments of 8 bits are (codes, exponents); those of 32 "
+                         "are values already")
     if _use_native(exp_avg[0]):
         return _EXT.adamw_decode(list(exp_avg), list(exp_avg_sq), dtype == torch.bfloat16)
     return (ref.adamw_decode(*exp_avg, True).to(dtype), ref.adamw_decode(*exp_avg_sq, False).to(dtype))

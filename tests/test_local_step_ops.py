@@ -305,3 +305,11 @@ def test_operators_under_vmap():
     # other transforms go through the plain operations
     assert torch.allclose(torch.func.grad(lambda w: n(x[0], w).sum())(w[0]),
                           torch.autograd.grad(n(x[0], leaves[1][0]).sum(), leaves[1])[0][0])
+
+
+def test_dequantize_refuses_moments_of_32_bits():
+    m, v, _ = ops.adamw_state(2, "cpu")
+    m8, v8, _ = ops.adamw_state(2, "cpu", 8)
+    for args in ((m, v), (m8, v), (m, v8)):
+        with pytest.raises(ValueError):
+            ops.adamw_dequantize(*args)
