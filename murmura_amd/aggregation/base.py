@@ -3,8 +3,8 @@
 Reference surface: murmura/aggregation/base.py:9-170. The reference aggregates
 CPU state dicts key-by-key with ``.item()`` host syncs per tensor; here every
 algorithm operates on flat state vectors ([P]) and stacked neighbor states
-([k, P]) so the hot math is a handful of single-kernel launches (SURVEY.md
-§2.9) and stays entirely on-device.
+([k, P]) so the hot math is a handful of single-kernel launches
+and stays entirely on-device.
 
 Statistics discipline: per-round scalars are kept as 0-dim device tensors in
 Python lists and only materialized to floats inside ``get_statistics()`` —
@@ -107,9 +107,8 @@ class EvalContext:
         return v / n, c.float() / n
 
     # ------------------------------------------------------ batched scoring
-    # UBAR stage-2 / EvidentialTrust / DMTT scoring
-    # ran m sequential copy_from_flat + forward per candidate per round. Here
-    # all k candidate states are evaluated in ONE vmapped forward
+    # UBAR stage-2 / EvidentialTrust / DMTT scoring by the serial path takes m
+    # sequential copy_from_flat + forward per round. Here all k candidate states are evaluated in ONE vmapped forward
     # (torch.func.functional_call over views into the stacked [k, P] tensor —
     # float buffers like BN running stats are part of the flat state, so each
     # candidate is evaluated with ITS OWN stats, matching the serial path).

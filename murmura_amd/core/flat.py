@@ -1,4 +1,4 @@
-"""Flat parameter buffers — the K13 design decision (SURVEY.md §2.9).
+"""Flat parameter buffers — the K13 design decision.
 
 Every node's float model state lives in ONE contiguous device tensor; the
 model's parameters and float buffers are views into it. This is what lets

@@ -1,6 +1,6 @@
 """Model zoo: MLPs/CNNs matching the reference's families and size ladder
 (reference: murmura/examples/leaf/models.py:12-216, datasets.py:204-297), plus
-the ResNet-18-sized benchmark CNN named by BASELINE.json config 2.
+the ResNet-18-sized CNN of the benchmark.
 
 All models are plain float modules; binding to flat buffers happens in
 FlatParamStore, dtype (fp32/bf16) is chosen by the node.
@@ -163,8 +163,8 @@ class BasicBlock(nn.Module):
 
 
 class ResNet18(nn.Module):
-    """ResNet-18 with a CIFAR-style 3x3 stem (~11.2M params) — the
-    "ResNet-18-sized CNN" of BASELINE.json config 2.
+    """ResNet-18 with a CIFAR-style 3x3 stem (~11.2M params), the
+    benchmark's model.
 
     ``norm="group"`` takes group norm (at most ``groups`` groups) in place of
     batch norm: no statistics over a batch, and none to be averaged between
@@ -194,7 +194,7 @@ class ResNet18(nn.Module):
 
 class WideMLP(nn.Module):
     """~100M-param MLP (in 4096 -> 12288 -> 4096 -> classes): the
-    bandwidth-bound Sketchguard showcase model (BASELINE.json config 4) —
+    bandwidth-bound Sketchguard showcase model —
     P ~ 100M floats means each neighbor state is 400 MB fp32 / 200 MB bf16
     on the xGMI wire."""
 

@@ -1,8 +1,8 @@
 """Op dispatch: hand-written CDNA4 HIP kernels on GPU, torch reference on CPU.
 
-Policy (per the build rules): when a tensor is on a ROCm device the native
-extension MUST be present and is always used — a silent eager fallback on the
-GPU box is a bug, so we raise instead. The torch implementations in
+Policy: when a tensor is on a ROCm device the native
+extension MUST be present and is always used — a silent eager fallback there
+is a bug, so we raise instead. The torch implementations in
 ``reference.py`` serve the CPU simulation backend and the numerics tests.
 
 Set MURMURA_DISABLE_NATIVE=1 to force the torch path everywhere (debug only).

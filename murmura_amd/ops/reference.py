@@ -1,7 +1,7 @@
 """Torch reference implementations of every hot op (the bit-level oracle).
 
 Each function here is the semantic definition of a HIP kernel in
-murmura_amd/ops/hip/ (kernel inventory: SURVEY.md §2.9 K1-K12). The GPU path
+murmura_amd/ops/hip/ (K1 to K18). The GPU path
 must match these within float tolerance; numerics tests compare the HIP kernel
 against the fp32 torch implementation of the same op.
 
