@@ -108,7 +108,8 @@ class EvalContext:
 
     # ------------------------------------------------------ batched scoring
     # UBAR stage-2 / EvidentialTrust / DMTT scoring by the serial path takes m
-    # sequential copy_from_flat + forward per round. Here all k candidate states are evaluated in ONE vmapped forward
+    # sequential copy_from_flat + forward per round. Here all k candidate
+    # states are evaluated in ONE vmapped forward
     # (torch.func.functional_call over views into the stacked [k, P] tensor —
     # float buffers like BN running stats are part of the flat state, so each
     # candidate is evaluated with ITS OWN stats, matching the serial path).
